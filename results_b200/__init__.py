@@ -12,6 +12,8 @@ re-designed for 8xB200 with NVLink 5 / NVSwitch):
   update transfer (raw / split+rANS), chunk-pipelined
 * ``encode`` / ``decode`` -- the LZC1 lossless float codec
 * ``pack_fp8`` / ``unpack_fp8`` -- e4m3 / e5m2 pair packing
+* ``token_logprobs`` / ``policy_loss`` / ``preference_loss`` / ``distill_loss``
+  -- the trainer's losses over the vocabulary, forward and backward
 """
 from __future__ import annotations
 
@@ -22,7 +24,8 @@ from .config import Config  # noqa: F401
 
 __all__ = ["Config", "Communicator", "init", "allreduce", "get_comm", "shutdown", "select_algo",
            "compressed_allreduce", "all_to_all", "send_weights", "recv_weights", "broadcast_weights",
-           "WeightTransfer", "encode", "decode", "pack_fp8", "unpack_fp8"]
+           "WeightTransfer", "encode", "decode", "pack_fp8", "unpack_fp8",
+           "token_logprobs", "policy_loss", "preference_loss", "distill_loss"]
 
 
 def __dir__():
@@ -59,4 +62,8 @@ def __getattr__(name):
         from .ops import fp8
 
         return getattr(fp8, name)
+    if name in ("token_logprobs", "policy_loss", "preference_loss", "distill_loss"):
+        from .ops import losses
+
+        return getattr(losses, name)
     raise AttributeError(name)

@@ -1,1 +1,1 @@
-"""Data transforms: split/rANS codec and fp8 packing (GPU kernels + CPU oracle)."""
+"""Data transforms (split/rANS codec, fp8 packing) and losses over the vocabulary."""

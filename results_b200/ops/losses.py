@@ -1,0 +1,574 @@
+"""Losses over the vocabulary: what an RL trainer, a preference trainer or a
+student computes between its output head and its backward pass.
+
+    logp = token_logprobs(logits, tokens)                      # rollout / reference log-probabilities
+    out = policy_loss(logits, tokens, old_logp, advantages, ref_logp=ref, kl_coef=0.02)
+    out = preference_loss(logits, tokens, ref_logp=ref)        # first half chosen, second half rejected
+    out = distill_loss(logits, teacher_ids, teacher_logits)    # the teacher's top entries
+    out.loss.backward()
+
+``logits`` is ``[..., vocab]`` in bf16, fp16 or fp32, ``tokens`` its leading
+shape in int32 or int64. Leading dimensions may have any strides (``logits[:, :-1]``
+is read in place); a vocabulary that is not contiguous is copied. A negative
+token marks a row that does not count (prompt, padding): its logits are not
+read, its outputs and its gradient are zero. The same holds for rows of weight
+zero. A token or teacher id beyond the vocabulary makes the row (and the loss) NaN.
+
+Sums and log-probabilities are held in 32 bits or more and a gradient is
+rounded once, to the logits' type. Results do not depend on timing: the same
+inputs give the same bits.
+
+On the GPU ``policy_loss`` and ``distill_loss`` write the gradient during the
+forward pass, while a row is still on the chip, for an upstream gradient of 1;
+the backward pass looks at the upstream on the device and computes the
+gradient anew, from the logits, if it is another (a loss divided by the number
+of micro batches, a loss scaler). Pass such a factor through ``denom`` instead
+to keep the cheaper way. The logits must not be changed before the backward
+pass. CUDA tensors run the kernels in csrc/lz_losses.cu on the current stream
+of their device; CPU tensors run the definitions in 64-bit torch operations.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple
+
+import torch
+
+from .. import _native, _native_sigs
+from ..utils.dtypes import LZ_BF16, LZ_F16, LZ_F32
+from ..utils.trace import traced
+
+LOGP, POLICY, DISTILL = 0, 1, 2
+MAX_TOP = 1024
+_HEAD, _PER_ROW = 2, 4  # doubles of the workspace (csrc/lz_losses.h)
+_DTYPES = {torch.float32: LZ_F32, torch.float16: LZ_F16, torch.bfloat16: LZ_BF16}
+_IDS = (torch.int64, torch.int32)
+
+_p, _l, _f, _d, _i = C.c_void_p, C.c_longlong, C.c_float, C.c_double, C.c_int
+
+
+class _LossArgs(C.Structure):  # struct LzLossArgs
+    _fields_ = [("logits", _p), ("outer_stride", _l), ("inner_stride", _l), ("inner", _l), ("rows", _l), ("vocab", _l),
+                ("grad", _p), ("ids", _p), ("teacher", _p), ("old_logp", _p), ("advantages", _p), ("ref_logp", _p),
+                ("weights", _p), ("denom_ptr", _p), ("upstream", _p), ("row_upstream", _p), ("loss", _p), ("logp", _p),
+                ("kl", _p), ("clipped", _p), ("work", _p), ("denom", _d), ("inv_temperature", _f), ("clip_low", _f),
+                ("clip_high", _f), ("kl_coef", _f), ("kind", _i), ("dtype", _i), ("ids64", _i), ("top", _i),
+                ("teacher_dtype", _i), ("device", _i), ("fresh", _i)]
+
+
+class _PairArgs(C.Structure):  # struct LzPairArgs
+    _fields_ = [("logp", _p), ("ids", _p), ("offsets", _p), ("ref_logp", _p), ("loss", _p), ("rewards", _p),
+                ("work", _p), ("rows", _l), ("pairs", _l), ("length", _l), ("beta", _d), ("smoothing", _d),
+                ("normalized", _i), ("ids64", _i), ("offsets64", _i), ("device", _i)]
+
+
+_native_sigs.add_cuda({
+    "lz_loss_forward": (_i, C.POINTER(_LossArgs), _p),
+    "lz_loss_backward": (_i, C.POINTER(_LossArgs), _p),
+    "lz_loss_pairs": (_i, C.POINTER(_PairArgs), _p),
+})
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor            # scalar
+    logp: torch.Tensor            # per token, no gradient
+    kl: torch.Tensor | None       # per token, no gradient; None without ref_logp
+    clipped: torch.Tensor         # per token: the clip is active
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor              # scalar
+    chosen_rewards: torch.Tensor    # per pair: beta (sum of logp - ref), no gradient
+    rejected_rewards: torch.Tensor
+
+
+class DistillLoss(NamedTuple):
+    loss: torch.Tensor  # scalar
+    kl: torch.Tensor    # per row, no gradient
+
+
+# ---- checks ---------------------------------------------------------------------------------------------
+
+
+def _check_logits(what: str, logits: torch.Tensor) -> None:
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"{what}: logits are {logits.dtype}; expected bfloat16, float16 or float32")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits of shape {tuple(logits.shape)} have no vocabulary")
+    if logits.shape[-1] > 2**31 - 1:
+        raise ValueError(f"{what}: a vocabulary of {logits.shape[-1]} entries is too large")
+    if logits.device.type not in ("cuda", "cpu"):
+        raise ValueError(f"{what}: device {logits.device} is not supported")
+
+
+def _check_ids(what: str, name: str, ids: torch.Tensor, shape, device) -> torch.Tensor:
+    if ids.dtype not in _IDS:
+        raise TypeError(f"{what}: {name} are {ids.dtype}; expected int64 or int32")
+    if tuple(ids.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} have shape {tuple(ids.shape)}; expected {tuple(shape)}")
+    if ids.device != device:
+        raise ValueError(f"{what}: {name} are on {ids.device}, the logits on {device}")
+    return ids.contiguous()
+
+
+def _check_rows(what: str, name: str, t: torch.Tensor | None, shape, device, any_type=False) -> torch.Tensor | None:
+    """A value per row (or sequence) as contiguous fp32."""
+    if t is None:
+        return None
+    if not (t.is_floating_point() or any_type) or t.is_complex():
+        raise TypeError(f"{what}: {name} is {t.dtype}; expected a floating-point type")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}; expected {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, the logits on {device}")
+    if t.requires_grad:
+        raise ValueError(f"{what}: {name} requires a gradient, and this loss gives none to it; detach it")
+    return t.to(torch.float32).contiguous()
+
+
+def _check_number(what: str, name: str, v, low: float, high: float = math.inf, open_low: bool = False) -> float:
+    v = float(v)
+    if not (v > low if open_low else v >= low) or v > high or math.isinf(v):
+        raise ValueError(f"{what}: {name} = {v} is out of range")
+    return v
+
+
+def _check_temperature(what: str, temperature) -> float:
+    t = _check_number(what, "temperature", temperature, 0.0, open_low=True)
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"{what}: temperature = {t} is out of range")
+    return t
+
+
+def _check_denom(what: str, denom, device):
+    """None, a positive number, or a tensor of one value on the logits' device."""
+    if denom is None or not isinstance(denom, torch.Tensor):
+        return None if denom is None else _check_number(what, "denom", denom, 0.0, open_low=True)
+    if denom.numel() != 1 or denom.is_complex():
+        raise ValueError(f"{what}: denom has shape {tuple(denom.shape)}; expected one number")
+    if denom.device != device:
+        raise ValueError(f"{what}: denom is on {denom.device}, the logits on {device}")
+    if denom.requires_grad:
+        raise ValueError(f"{what}: denom requires a gradient, and this loss gives none to it; detach it")
+    return denom.to(torch.float32)
+
+
+# ---- native calls ---------------------------------------------------------------------------------------
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _rows_of(x: torch.Tensor):
+    """(tensor, rows, inner, outer stride, inner stride): row r starts at
+    (r // inner) * outer stride + (r % inner) * inner stride. Copies only where
+    two strides and a contiguous vocabulary cannot say it."""
+    lead = x.shape[:-1]
+    rows = math.prod(lead)
+    if x.stride(-1) != 1 and x.shape[-1] > 1 or len(lead) > 2:
+        x = x.contiguous()
+    if len(lead) > 2 or x.is_contiguous():
+        return x, rows, max(1, rows), 0, x.shape[-1]
+    if len(lead) == 2:
+        return x, rows, max(1, lead[1]), x.stride(0), x.stride(1)
+    return x, rows, max(1, rows), 0, x.stride(0) if lead else 0
+
+
+def _args(kind: int, logits: torch.Tensor, ids: torch.Tensor, work: torch.Tensor, temperature: float) -> _LossArgs:
+    x, rows, inner, outer_stride, inner_stride = _rows_of(logits)
+    a = _LossArgs(kind=kind, logits=x.data_ptr(), rows=rows, inner=inner, outer_stride=outer_stride,
+                  inner_stride=inner_stride, vocab=x.shape[-1], ids=ids.data_ptr(), ids64=ids.dtype == torch.int64,
+                  work=work.data_ptr(), inv_temperature=1.0 / temperature, dtype=_DTYPES[x.dtype], device=x.device.index)
+    a.copied = x  # alive as long as the arguments are
+    return a
+
+
+def _launch(fn: str, a, device, what: str) -> None:
+    stream = torch.cuda.current_stream(device).cuda_stream
+    _native.check(getattr(_native.cuda(), fn)(C.byref(a), stream), what)
+
+
+def _work(logits: torch.Tensor) -> torch.Tensor:
+    rows = math.prod(logits.shape[:-1])
+    return torch.empty(_HEAD + _PER_ROW * rows, dtype=torch.float64, device=logits.device)
+
+
+def _grad_buffer(logits: torch.Tensor) -> torch.Tensor:
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+def _set_denom(a: _LossArgs, denom) -> None:
+    if isinstance(denom, torch.Tensor):
+        a.denom_ptr = denom.data_ptr()
+    else:
+        a.denom = -1.0 if denom is None else denom
+
+
+def _logprobs_forward(logits, tokens, temperature):
+    logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+    work = _work(logits)
+    a = _args(LOGP, logits, tokens, work, temperature)
+    a.logp = logp.data_ptr()
+    _launch("lz_loss_forward", a, logits.device, "token log-probabilities")
+    return logp, work
+
+
+def _logprobs_backward(logits, tokens, work, temperature, row_upstream, upstream=None):
+    grad = _grad_buffer(logits)
+    a = _args(LOGP, logits, tokens, work, temperature)
+    a.grad, a.row_upstream, a.upstream, a.fresh = grad.data_ptr(), row_upstream.data_ptr(), _ptr(upstream), 1
+    _launch("lz_loss_backward", a, logits.device, "token log-probabilities, backward")
+    return grad
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature):
+        logp, work = _logprobs_forward(logits, tokens, temperature)
+        ctx.save_for_backward(logits, tokens, work)
+        ctx.temperature = temperature
+        return logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        logits, tokens, work = ctx.saved_tensors
+        g = g.to(torch.float32).contiguous()
+        return _logprobs_backward(logits, tokens, work, ctx.temperature, g), None, None
+
+
+def _policy_forward(logits, tokens, rows, p, grad):
+    """rows: old_logp, advantages, ref_logp, weights; p: the loss's numbers."""
+    old, adv, ref, weights = rows
+    dev = logits.device
+    work = _work(logits)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    kl = None if ref is None else torch.empty_like(logp)
+    clipped = torch.empty(tokens.shape, dtype=torch.bool, device=dev)
+    a = _args(POLICY, logits, tokens, work, p["temperature"])
+    a.old_logp, a.advantages, a.ref_logp, a.weights = _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights)
+    a.loss, a.logp, a.kl, a.clipped, a.grad = _ptr(loss), _ptr(logp), _ptr(kl), _ptr(clipped), _ptr(grad)
+    a.clip_low, a.clip_high, a.kl_coef = p["clip_low"], p["clip_high"], p["kl_coef"]
+    _set_denom(a, p["denom"])
+    _launch("lz_loss_forward", a, dev, "policy loss")
+    return loss, logp, kl, clipped, work
+
+
+def _distill_forward(logits, ids, teacher, weights, p, grad):
+    dev = logits.device
+    work = _work(logits)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    a = _args(DISTILL, logits, ids, work, p["temperature"])
+    a.teacher, a.teacher_dtype, a.top, a.weights = _ptr(teacher), _DTYPES[teacher.dtype], ids.shape[-1], _ptr(weights)
+    a.loss, a.kl, a.grad = _ptr(loss), _ptr(kl), _ptr(grad)
+    _set_denom(a, p["denom"])
+    _launch("lz_loss_forward", a, dev, "distillation loss")
+    return loss, kl, work
+
+
+def _scalar_backward(ctx, kind, g, logits, ids, work, teacher=None):
+    """The gradient that the forward pass left, for upstream `g`. It is handed
+    out once: a second pass over a retained graph writes into memory of its own."""
+    grad, ctx.grad = ctx.grad, None
+    a = _args(kind, logits, ids, work, ctx.p["temperature"])
+    a.fresh = grad is None
+    if grad is None:
+        grad = _grad_buffer(logits)
+    if teacher is not None:
+        a.teacher, a.teacher_dtype, a.top = _ptr(teacher), _DTYPES[teacher.dtype], ids.shape[-1]
+    g = g.to(torch.float32)
+    a.grad, a.upstream = grad.data_ptr(), g.data_ptr()
+    _launch("lz_loss_backward", a, logits.device, "loss, backward")
+    return grad
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, rows, p):
+        ctx.grad, ctx.p = _grad_buffer(logits), p
+        loss, logp, kl, clipped, work = _policy_forward(logits, tokens, rows, p, ctx.grad)
+        ctx.save_for_backward(logits, tokens, work)
+        ctx.mark_non_differentiable(*(t for t in (logp, kl, clipped) if t is not None))
+        ctx.set_materialize_grads(False)
+        return loss, logp, kl, clipped
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, *_):
+        if g is None:
+            return None, None, None, None
+        return _scalar_backward(ctx, POLICY, g, *ctx.saved_tensors), None, None, None
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, weights, p):
+        ctx.grad, ctx.p = _grad_buffer(logits), p
+        loss, kl, work = _distill_forward(logits, ids, teacher, weights, p, ctx.grad)
+        ctx.save_for_backward(logits, ids, work, teacher)
+        ctx.mark_non_differentiable(kl)
+        ctx.set_materialize_grads(False)
+        return loss, kl
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, *_):
+        if g is None:
+            return None, None, None, None, None
+        return _scalar_backward(ctx, DISTILL, g, *ctx.saved_tensors), None, None, None, None
+
+
+def _preference_forward(logits, tokens, ref, offsets, p):
+    logp, work = _logprobs_forward(logits, tokens, p["temperature"])
+    dev, pairs, rows = logits.device, p["pairs"], tokens.numel()
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    rewards = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
+    pair_work = torch.empty(1 + pairs + (rows + 1) // 2, dtype=torch.float64, device=dev)
+    a = _PairArgs(logp=_ptr(logp), ids=_ptr(tokens), offsets=_ptr(offsets), ref_logp=_ptr(ref), loss=_ptr(loss),
+                  rewards=_ptr(rewards), work=_ptr(pair_work), rows=rows, pairs=pairs, length=p["length"],
+                  beta=p["beta"], smoothing=p["label_smoothing"], normalized=p["length_normalized"],
+                  ids64=tokens.dtype == torch.int64, offsets64=offsets is not None and offsets.dtype == torch.int64,
+                  device=dev.index)
+    _launch("lz_loss_pairs", a, dev, "preference loss")
+    slope = pair_work[1 + pairs:].view(torch.float32)
+    return loss, rewards, work, slope
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, ref, offsets, p):
+        loss, rewards, work, slope = _preference_forward(logits, tokens, ref, offsets, p)
+        ctx.save_for_backward(logits, tokens, work, slope)
+        ctx.temperature = p["temperature"]
+        ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
+        return loss, rewards
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, *_):
+        if g is None:
+            return None, None, None, None, None
+        logits, tokens, work, slope = ctx.saved_tensors
+        g = g.to(torch.float32)
+        return _logprobs_backward(logits, tokens, work, ctx.temperature, slope, g), None, None, None, None
+
+
+# ---- the definitions (CPU tensors) -----------------------------------------------------------------------
+
+
+def _cpu_logp(logits, ids, counted, temperature):
+    """Log-probabilities of ids [rows, k] in 64 bits; rows that do not count are not looked at."""
+    v = logits.shape[-1]
+    z = torch.where(counted[:, None], logits.reshape(-1, v).double(), 0.0) / temperature
+    logp = torch.log_softmax(z, -1).gather(1, ids.clamp(0, v - 1).long())
+    return torch.where((ids >= v) & counted[:, None], math.nan, logp)
+
+
+def _cpu_scale(weights, counted, denom):
+    w = counted.double() if weights is None else torch.where(counted, weights.reshape(-1).double(), 0.0)
+    d = w.sum() if denom is None else torch.as_tensor(denom, dtype=torch.float64).reshape(())
+    return torch.where(d <= 0, 0.0, w / d)
+
+
+def _cpu_token_logprobs(logits, tokens, temperature):
+    y = tokens.reshape(-1)
+    logp = _cpu_logp(logits, y[:, None], y >= 0, temperature)[:, 0]
+    return torch.where(y >= 0, logp, 0.0).float().view(tokens.shape)
+
+
+def _cpu_policy_loss(logits, tokens, rows, p):
+    old, adv, ref, weights = (None if t is None else t.reshape(-1).double() for t in rows)
+    y = tokens.reshape(-1)
+    scale = _cpu_scale(weights, y >= 0, p["denom"])
+    counted = (y >= 0) & (weights != 0) if weights is not None else y >= 0
+    logp = torch.where(counted, _cpu_logp(logits, y[:, None], counted, p["temperature"])[:, 0], 0.0)
+    ratio = torch.where(counted, logp - old, 0.0).exp()
+    low, high = 1.0 - p["clip_low"], 1.0 + p["clip_high"]
+    clipped = (((adv > 0) & (ratio > high)) | ((adv < 0) & (ratio < low))) & counted
+    each = -adv * torch.where(clipped, torch.where(adv > 0, high, low), ratio)
+    kl = None
+    if ref is not None:
+        d = torch.where(counted, ref - logp, 0.0)
+        kl = d.expm1() - d
+        each = each + p["kl_coef"] * kl
+        kl = kl.detach().float().view(tokens.shape)
+    loss = torch.where(counted, each * scale, 0.0).sum().float()
+    return loss, logp.detach().float().view(tokens.shape), kl, clipped.view(tokens.shape)
+
+
+def _cpu_distill_loss(logits, ids, teacher, weights, p):
+    n, k = math.prod(ids.shape[:-1]), ids.shape[-1]
+    ids, t = ids.reshape(n, k), teacher.reshape(n, k).double() / p["temperature"]
+    there = ids >= 0
+    t = torch.where(there, t, -math.inf)
+    counted = torch.ones(n, dtype=torch.bool) if weights is None else weights.reshape(-1) != 0
+    some = t.amax(1) != -math.inf
+    logq = torch.log_softmax(torch.where(some[:, None], t, 0.0), 1)
+    q = torch.where(there & some[:, None], logq.exp(), 0.0)
+    logp = _cpu_logp(logits, ids, counted & some, p["temperature"])
+    kl = torch.where(q > 0, q * (logq - logp), 0.0)
+    kl = torch.where(q.isnan() | (ids >= logits.shape[-1]), math.nan, kl).sum(1)
+    kl = torch.where(counted, kl, 0.0)
+    loss = (kl * _cpu_scale(weights, torch.ones_like(counted), p["denom"])).sum().float()
+    return loss, kl.detach().float().view(logits.shape[:-1])
+
+
+def _cpu_preference_loss(logits, tokens, ref, offsets, p):
+    y, pairs = tokens.reshape(-1), p["pairs"]
+    logp = torch.where(y >= 0, _cpu_logp(logits, y[:, None], y >= 0, p["temperature"])[:, 0], 0.0)
+    ends = [s * p["length"] for s in range(2 * pairs + 1)] if offsets is None else offsets.tolist()
+    sums = []
+    for a, b in zip(ends, ends[1:]):
+        if not 0 <= a <= b <= y.numel():
+            sums.append(torch.tensor(math.nan, dtype=torch.float64))
+            continue
+        count = max(1, int((y[a:b] >= 0).sum())) if p["length_normalized"] else 1
+        sums.append(logp[a:b].sum() / count)
+    r = p["beta"] * (torch.stack(sums) - (0.0 if ref is None else ref.double()))
+    h, eps = r[:pairs] - r[pairs:], p["label_smoothing"]
+    loss = -((1 - eps) * torch.nn.functional.logsigmoid(h) + eps * torch.nn.functional.logsigmoid(-h))
+    return loss.mean().float(), r.detach().float()
+
+
+# ---- public entry points ---------------------------------------------------------------------------------
+
+
+def _needs_grad(logits: torch.Tensor) -> bool:
+    return logits.requires_grad and torch.is_grad_enabled()
+
+
+@traced("token_logprobs")
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0) -> torch.Tensor:
+    """log softmax(logits / temperature) at ``tokens``, fp32, differentiable in the logits."""
+    what = "token_logprobs"
+    _check_logits(what, logits)
+    tokens = _check_ids(what, "tokens", tokens, logits.shape[:-1], logits.device)
+    temperature = _check_temperature(what, temperature)
+    if not logits.is_cuda:
+        return _cpu_token_logprobs(logits, tokens, temperature)
+    if _needs_grad(logits):
+        return _TokenLogprobs.apply(logits, tokens, temperature)
+    return _logprobs_forward(logits, tokens, temperature)[0]
+
+
+@traced("policy_loss")
+def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
+                ref_logp: torch.Tensor | None = None, weights: torch.Tensor | None = None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0, denom=None) -> PolicyLoss:
+    """Clipped policy loss with a KL term to a reference policy:
+
+        ratio = exp(logp - old_logp)
+        each  = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef kl
+        kl    = exp(ref_logp - logp) - (ref_logp - logp) - 1
+        loss  = sum(weights each) / denom
+
+    ``old_logp``, ``advantages``, ``ref_logp`` and ``weights`` (a mask or
+    factors) have the tokens' shape. ``denom`` is a number or a one-element
+    tensor on the device (the token count over all micro batches or ranks);
+    without it, the sum of the weights of the rows that count. Where that is
+    not positive, loss and gradient are zero."""
+    what, dev, shape = "policy_loss", logits.device, logits.shape[:-1]
+    _check_logits(what, logits)
+    tokens = _check_ids(what, "tokens", tokens, shape, dev)
+    if ref_logp is None and kl_coef:
+        raise ValueError("policy_loss: kl_coef without ref_logp")
+    rows = (_check_rows(what, "old_logp", old_logp, shape, dev), _check_rows(what, "advantages", advantages, shape, dev),
+            _check_rows(what, "ref_logp", ref_logp, shape, dev),
+            _check_rows(what, "weights", weights, shape, dev, any_type=True))
+    if rows[0] is None or rows[1] is None:
+        raise ValueError("policy_loss: old_logp and advantages are needed")
+    p = {"clip_low": _check_number(what, "clip_low", clip_low, 0.0, 1.0),
+         "clip_high": _check_number(what, "clip_high", clip_high, 0.0),
+         "kl_coef": _check_number(what, "kl_coef", kl_coef, 0.0),
+         "temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
+    if not logits.is_cuda:
+        return PolicyLoss(*_cpu_policy_loss(logits, tokens, rows, p))
+    if _needs_grad(logits):
+        return PolicyLoss(*_PolicyLoss.apply(logits, tokens, rows, p))
+    return PolicyLoss(*_policy_forward(logits, tokens, rows, p, None)[:4])
+
+
+@traced("preference_loss")
+def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, *, ref_logp: torch.Tensor | None = None,
+                    cu_seqlens: torch.Tensor | None = None, beta: float = 0.1, label_smoothing: float = 0.0,
+                    length_normalized: bool = False, temperature: float = 1.0) -> PreferenceLoss:
+    """Preference loss on paired log ratios. The batch holds 2 P sequences, the
+    P chosen ones first, then their rejected partners in the same order:
+    ``logits`` ``[2 P, length, vocab]`` and ``tokens`` ``[2 P, length]``, or
+    packed ``[rows, vocab]`` and ``[rows]`` with ``cu_seqlens`` ``[2 P + 1]``
+    (rows outside of it get a zero gradient; offsets that do not rise within
+    the rows make the loss NaN).
+
+        s    = sum of a sequence's log-probabilities (mean where length_normalized)
+        h    = beta ((s_chosen - ref_chosen) - (s_rejected - ref_rejected))
+        loss = mean(-(1 - eps) log sigmoid(h) - eps log sigmoid(-h)),  eps = label_smoothing
+
+    ``ref_logp`` ``[2 P]`` holds the reference model's s; without it, zeros."""
+    what, dev = "preference_loss", logits.device
+    _check_logits(what, logits)
+    if cu_seqlens is None:
+        if logits.dim() != 3 or logits.shape[0] < 2 or logits.shape[0] % 2:
+            raise ValueError(f"preference_loss: logits of shape {tuple(logits.shape)}; expected [2 pairs, length, vocab], "
+                             "or [rows, vocab] with cu_seqlens")
+        sequences, length = logits.shape[0], logits.shape[1]
+    else:
+        if logits.dim() != 2:
+            raise ValueError(f"preference_loss: packed logits of shape {tuple(logits.shape)}; expected [rows, vocab]")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 3 or cu_seqlens.numel() % 2 == 0:
+            raise ValueError(f"preference_loss: cu_seqlens of shape {tuple(cu_seqlens.shape)}; expected [2 pairs + 1]")
+        cu_seqlens = _check_ids(what, "cu_seqlens", cu_seqlens, cu_seqlens.shape, dev)
+        sequences, length = cu_seqlens.numel() - 1, 0
+    tokens = _check_ids(what, "tokens", tokens, logits.shape[:-1], dev)
+    ref = _check_rows(what, "ref_logp", ref_logp, (sequences,), dev)
+    p = {"pairs": sequences // 2, "length": length, "beta": _check_number(what, "beta", beta, 0.0),
+         "label_smoothing": _check_number(what, "label_smoothing", label_smoothing, 0.0, 1.0),
+         "length_normalized": bool(length_normalized), "temperature": _check_temperature(what, temperature)}
+    if not logits.is_cuda:
+        loss, rewards = _cpu_preference_loss(logits, tokens, ref, cu_seqlens, p)
+    elif _needs_grad(logits):
+        loss, rewards = _PreferenceLoss.apply(logits, tokens, ref, cu_seqlens, p)
+    else:
+        loss, rewards = _preference_forward(logits, tokens, ref, cu_seqlens, p)[:2]
+    return PreferenceLoss(loss, rewards[:p["pairs"]], rewards[p["pairs"]:])
+
+
+@traced("distill_loss")
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                 weights: torch.Tensor | None = None, temperature: float = 1.0, denom=None) -> DistillLoss:
+    """Distillation from a teacher's top entries (up to 1024 a row):
+
+        q    = softmax(teacher_logits / temperature) over the row's entries
+        kl   = sum_k q_k (log q_k - log softmax(logits / temperature)[id_k])
+        loss = sum(weights kl) / denom
+
+    ``teacher_ids`` and ``teacher_logits`` (logits or log-probabilities, bf16,
+    fp16 or fp32) are ``[..., K]``; a negative id is padding. An id that stands
+    in a row twice counts with both shares. A row without entries has loss and
+    gradient zero. ``weights`` and ``denom`` as in :func:`policy_loss`; without
+    ``denom``, the sum of the weights of all rows."""
+    what, dev = "distill_loss", logits.device
+    _check_logits(what, logits)
+    if teacher_ids.dim() < 1 or not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
+        raise ValueError(f"distill_loss: teacher_ids of shape {tuple(teacher_ids.shape)}; expected 1 to {MAX_TOP} entries a row")
+    shape = logits.shape[:-1]
+    ids = _check_ids(what, "teacher_ids", teacher_ids, (*shape, teacher_ids.shape[-1]), dev)
+    if teacher_logits.dtype not in _DTYPES:
+        raise TypeError(f"distill_loss: teacher_logits are {teacher_logits.dtype}; expected bfloat16, float16 or float32")
+    if teacher_logits.shape != ids.shape or teacher_logits.device != dev:
+        raise ValueError(f"distill_loss: teacher_logits {tuple(teacher_logits.shape)} on {teacher_logits.device} do not "
+                         f"match teacher_ids {tuple(ids.shape)} on {dev}")
+    if teacher_logits.requires_grad:
+        raise ValueError("distill_loss: teacher_logits require a gradient, and this loss gives none to them; detach them")
+    teacher = teacher_logits.contiguous()
+    weights = _check_rows(what, "weights", weights, shape, dev, any_type=True)
+    p = {"temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
+    if not logits.is_cuda:
+        return DistillLoss(*_cpu_distill_loss(logits, ids, teacher, weights, p))
+    if _needs_grad(logits):
+        return DistillLoss(*_DistillLoss.apply(logits, ids, teacher, weights, p))
+    return DistillLoss(*_distill_forward(logits, ids, teacher, weights, p, None)[:2])
