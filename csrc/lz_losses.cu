@@ -12,6 +12,9 @@
 // exponential. Sums run in 32 bits a thread; what is per row (lse2, the slope,
 // the loss) in 64 bits, since a log-probability enters the KL term and the
 // ratio as a difference and costs nothing per element.
+#include <atomic>
+#include <type_traits>
+
 #include "lz_common.cuh"
 #include "lz_internal.h"
 #include "lz_losses.h"
@@ -285,13 +288,25 @@ LZ_DEV float load_any(const void* p, int dtype, long long i) {
 
 template <typename T>
 LZ_DEV const T* row_of(const LzLossArgs& a, long long r) {
-  return static_cast<const T*>(a.logits) + (r / a.inner) * a.outer_stride + (r % a.inner) * a.inner_stride;
+  const T* x = static_cast<const T*>(a.logits);
+  if (a.inner == a.rows) return x + r * a.inner_stride;
+  return x + (r / a.inner) * a.outer_stride + (r % a.inner) * a.inner_stride;
 }
 
 // The parts of `work`.
 LZ_DEV double2* work_norm(const LzLossArgs& a) { return reinterpret_cast<double2*>(a.work + LZ_LOSS_WORK_HEAD); }
 LZ_DEV double* work_slope(const LzLossArgs& a) { return a.work + LZ_LOSS_WORK_HEAD + 2 * a.rows; }
 LZ_DEV double* work_loss(const LzLossArgs& a) { return a.work + LZ_LOSS_WORK_HEAD + 3 * a.rows; }
+LZ_DEV int* work_order(const LzLossArgs& a) { return reinterpret_cast<int*>(a.work + LZ_LOSS_WORK_HEAD + 4 * a.rows); }
+LZ_DEV unsigned* work_ticket(const LzLossArgs& a) { return reinterpret_cast<unsigned*>(a.work + 1); }
+LZ_DEV int* work_active(const LzLossArgs& a) { return reinterpret_cast<int*>(a.work + 1) + 1; }
+
+// Whether a row counts: its token is not negative and its weight not zero.
+template <int KIND>
+LZ_DEV bool row_counts(const LzLossArgs& a, long long r) {
+  return (KIND == LZ_LOSS_DISTILL || load_id(a.ids, a.ids64, r) >= 0) &&
+         (KIND == LZ_LOSS_LOGP || !a.weights || a.weights[r] != 0.f);
+}
 
 // The teacher's list of one row in shared memory.
 struct Top {
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0)
-    last = atomicAdd(reinterpret_cast<unsigned*>(a.work + 1), 1u) == gridDim.x - 1;
+    last = atomicAdd(work_ticket(a), 1u) == gridDim.x - 1;
   __syncthreads();
   if (!last) return;
   __threadfence();
@@ -466,24 +481,51 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   if (threadIdx.x == 0) *a.loss = (float)s;
 }
 
-// 1 / denominator (0 where that is not positive: nothing counts) and the ticket.
-__global__ void __launch_bounds__(kThreads) head_kernel(const __grid_constant__ LzLossArgs a) {
+// 1 / denominator (0 where that is not positive: nothing counts), the ticket and,
+// where `order` is set, the rows that count in front of those that do not, each
+// in their order: taken in turns, every cluster of stream_kernel gets as many.
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) head_kernel(const __grid_constant__ LzLossArgs a, bool order) {
   __shared__ double red[kWarps];
+  __shared__ int counts[2][kWarps];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   double s = 0.0;
-  if (a.denom_ptr) {
-    s = (double)*a.denom_ptr;
-  } else if (a.denom >= 0.0) {
-    s = a.denom;
-  } else {
-    for (long long r = threadIdx.x; r < a.rows; r += kThreads)
-      if (a.kind == LZ_LOSS_DISTILL || load_id(a.ids, a.ids64, r) >= 0) s += a.weights ? (double)a.weights[r] : 1.0;
-    s = block_sum(s, red);
+  if (KIND != LZ_LOSS_LOGP) {
+    if (a.denom_ptr) {
+      s = (double)*a.denom_ptr;
+    } else if (a.denom >= 0.0) {
+      s = a.denom;
+    } else {
+      for (long long r = threadIdx.x; r < a.rows; r += kThreads)
+        if (KIND == LZ_LOSS_DISTILL || load_id(a.ids, a.ids64, r) >= 0) s += a.weights ? (double)a.weights[r] : 1.0;
+      s = block_sum(s, red);
+    }
   }
   if (threadIdx.x == 0) {
     a.work[0] = s > 0.0 || s != s ? 1.0 / s : 0.0;
-    *reinterpret_cast<unsigned*>(a.work + 1) = 0u;
-    if (a.rows == 0) *a.loss = 0.f;
+    *work_ticket(a) = 0u;
+    if (KIND != LZ_LOSS_LOGP && a.rows == 0) *a.loss = 0.f;
   }
+  if (!order) return;
+  const int n = (int)a.rows;
+  int front = 0, back = 0;  // rows placed at either end
+  for (int first = 0, k = 0; first < n; first += kThreads, k ^= 1) {
+    const int r = first + threadIdx.x;
+    const bool counts_ = r < n && row_counts<KIND>(a, r);
+    const unsigned m = __ballot_sync(~0u, counts_);
+    if (lane == 0) counts[k][warp] = __popc(m);
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      before += w < warp ? counts[k][w] : 0;
+      all += counts[k][w];
+    }
+    before += __popc(m & ((1u << lane) - 1));
+    if (r < n) work_order(a)[counts_ ? front + before : n - 1 - (back + (int)threadIdx.x - before)] = r;
+    front += all;
+    back += min(kThreads, n - first) - all;
+  }
+  if (threadIdx.x == 0) *work_active(a) = front;
 }
 
 // The gradient from the rows' saved sums and slopes. POLICY and DISTILL: where
@@ -514,6 +556,750 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
     else if (y < a.vocab) row_sparse_token<T>(a, x, out, y, slope, n, c);
     __syncthreads();
   }
+}
+
+// ---------------------------------------------------------------------------
+// Large vocabularies: a cluster of CTAs a row, each with a slice of it.
+//
+// A row goes through shared memory once. One warp streams the slices of the
+// cluster's rows into a ring of chunks by bulk copies and runs ahead as far as
+// the ring has room. W warps take a chunk's part of the row's sum, and for the
+// gradient take the chunks a second time, from shared memory, and hand each back
+// to the ring. So HBM sees a row read once and its gradient written once, and
+// reads of the next row run under the writes of this one. One more warp keeps
+// what is per row off that path: it joins the warps' sums, exchanges them with
+// the cluster's CTAs through distributed shared memory, works out the row's
+// scalars from values fetched a row ahead (and the teacher's list), writes the
+// row's outputs, and puts the few entries with t_j != 0 over the dense gradient
+// once that is written. While it does, the W warps take the first chunks of the
+// next row, as many as fit beside this one.
+// ---------------------------------------------------------------------------
+
+constexpr int kMaxSlots = 64;
+constexpr int kMaxCluster = 8;
+constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of every wait
+
+struct StreamPlan {
+  int slots;    // of the ring, a chunk each
+  int early;    // chunks of the next row taken before this one's gradient
+  int ordered;  // rows by work_order; otherwise one row a cluster
+  int hash;     // entries of the hash table of DISTILL, a power of two
+};
+
+struct RowParams {
+  float xy, adv;
+  double old_logp2, ref_logp2;  // base 2
+  double weight;  // over the denominator
+  int token;      // -1: beyond the vocabulary
+  float slope;    // DISTILL
+  double q_logq, q_z, q_sum;  // DISTILL: sums over the list (z in base 2)
+};
+
+// Which row, and this CTA's slice of it.
+struct RowHead {
+  long long row;  // -1: no more
+  int lead, vecs, first, count, chunks;
+};
+
+// What the dense gradient of a row takes: f 2^((x - base) c - ref).
+struct RowDense {
+  float f, base, ref;
+};
+
+// The teacher's list of a row: entries and, with equal ids joined, what the gradient takes from them.
+struct TopView {
+  int* id;
+  float *z, *q, *share;  // share < 0: another entry of the same id has it
+};
+
+// Both rows' lists (id, z, q, share) and the hash table.
+__host__ __device__ inline int list_bytes(int kind, int top, int hash) {
+  return kind == LZ_LOSS_DISTILL ? (top * 32 + hash * 4 + 127) / 128 * 128 : 0;
+}
+
+struct alignas(128) StreamShared {
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t parts[2], peers[2], dense[2];  // of every other row
+  float2 warp_part[2][16];
+  float2 peer_part[2][kMaxCluster];
+  RowHead heads[4];
+  RowDense row_dense[2];
+  RowParams params;
+  int failed;
+};
+
+LZ_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+LZ_DEV uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+LZ_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+LZ_DEV void mbar_arrive(uint64_t* bar) {
+  asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.shared::cta.b64 t, [%0];\n\t}" ::"r"(smem_addr(bar)) : "memory");
+}
+// Stores v at `slot` of CTA `rank`'s shared memory and arrives at its `bar`.
+LZ_DEV void send_to_peer(float2* slot, float2 v, uint64_t* bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 s, b;\n\t"
+      "mapa.shared::cluster.u32 s, %0, %2;\n\t"
+      "mapa.shared::cluster.u32 b, %1, %2;\n\t"
+      "st.shared::cluster.v2.f32 [s], {%3, %4};\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [b];\n\t}" ::"r"(smem_addr(slot)),
+      "r"(smem_addr(bar)), "r"(rank), "f"(v.x), "f"(v.y)
+      : "memory");
+}
+// Waits for phase `parity` of `bar`, 4 s at most. A wait that gives up sets
+// `failed`, and the CTA's other waits then return at once: the kernel runs to its
+// end and leaves NaN.
+template <bool CLUSTER>
+LZ_DEV void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  unsigned long long began = 0;
+  for (uint32_t it = 0; it < 0xffffffffu; ++it) {
+    uint32_t done;
+    if (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(smem_addr(bar)), "r"(parity)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(smem_addr(bar)), "r"(parity)
+          : "memory");
+    if (done || *failed) return;
+    if (it % 64 == 63) {
+      const unsigned long long now = globaltimer();
+      if (!began) began = now;
+      if (now - began > kWaitNs) break;
+    }
+  }
+  *failed = 1;
+}
+
+// Two fp32 operations an instruction.
+LZ_DEV uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+LZ_DEV void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+LZ_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+LZ_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+LZ_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// The largest element of a vector; NaN only if all are.
+template <typename T>
+LZ_DEV float vector_max(uint4 v);
+template <>
+LZ_DEV float vector_max<float>(uint4 v) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+template <>
+LZ_DEV float vector_max<__nv_bfloat16>(uint4 v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(m.x, m.y);
+}
+template <>
+LZ_DEV float vector_max<__half>(uint4 v) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+  const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(m.x, m.y);
+}
+
+template <typename T>
+LZ_DEV void unpack_pairs(uint4 v, uint64_t* p) {
+  float f[Elem<T>::N];
+  Elem<T>::unpack(v, f);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N / 2; ++i) p[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+
+// A rank's share of a row: vectors [first, first + count) of those between the
+// 16-byte borders; the single elements outside of these are rank 0's.
+template <typename T>
+LZ_DEV RowHead slice_of(const T* x, long long row, long long vocab, uint32_t rank, uint32_t ranks, int chunk_vecs) {
+  const Split<T> sp(x, vocab);
+  RowHead h;
+  h.row = row, h.lead = sp.lead, h.vecs = sp.vecs;
+  const int per = (sp.vecs + (int)ranks - 1) / (int)ranks;
+  h.first = min((int)rank * per, sp.vecs);
+  h.count = min(per, sp.vecs - h.first);
+  h.chunks = (h.count + chunk_vecs - 1) / chunk_vecs;
+  return h;
+}
+
+// Index of the t-th single element, or -1.
+template <typename T>
+LZ_DEV long long single_of(const RowHead& h, int t, long long vocab) {
+  const long long tail = h.lead + (long long)h.vecs * Elem<T>::N;
+  if (t < h.lead) return t;
+  return t - h.lead < vocab - tail ? tail + t - h.lead : -1;
+}
+
+// log2 of a sum as an integer and a part in [-1/2, 1/2], so that neither is rounded away.
+LZ_DEV void log2_parts(float s, float* whole, float* part) {
+  const int bits = __float_as_int(s), e = (bits - 0x3f3504f3) >> 23;  // mantissa in [1/sqrt 2, sqrt 2)
+  const bool normal = s >= 0x1p-126f && s < INFINITY;
+  *whole = normal ? (float)e : 0.f;
+  *part = log2f(normal ? __int_as_float(bits - (e << 23)) : s);
+}
+
+// A row's normaliser: p_j = 2^((x_j - base) c - ref) / sum.
+struct RowSum {
+  float base, ref, sum;
+  LZ_DEV Norm norm() const {
+    float whole, part;
+    log2_parts(sum, &whole, &part);
+    return {base, (double)ref + (double)whole + (double)part};
+  }
+};
+
+// What a POLICY row's scalars give; logp2: the token's log-probability in base 2.
+struct PolicyOut {
+  float ratio, slope;
+  bool clipped;
+};
+LZ_DEV PolicyOut policy_out(const LzLossArgs& a, const RowParams& p, double logp2) {
+  PolicyOut o;
+  o.ratio = exp2f((float)(logp2 - p.old_logp2));
+  o.clipped = (p.adv > 0.f && o.ratio > 1.f + a.clip_high) || (p.adv < 0.f && o.ratio < 1.f - a.clip_low);
+  float slope = o.clipped ? 0.f : -p.adv * o.ratio;
+  if (a.ref_logp) slope -= a.kl_coef * expm1f((float)((p.ref_logp2 - logp2) * kLn2));
+  o.slope = (float)(p.weight * (double)slope);
+  return o;
+}
+
+// (max, sum) over the `n` lanes' values, n a power of two; the same in every lane.
+LZ_DEV void lanes_join(float& m, float& s, int n) {
+  float top = m;
+  for (int o = n / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  s *= m == -INFINITY ? 1.f : exp2_fast(m - top);  // a sum without a maximum is 0 or NaN
+  for (int o = n / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  m = top;
+}
+
+// Maximum and sum of a row whose scaled maximum is beyond 32 bits, by one warp.
+template <typename T>
+LZ_DEV RowSum slow_sum(const T* x, long long n, float c) {
+  const int lane = threadIdx.x % 32;
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 8
+  for (long long i = lane; i < n; i += 32) m = fmaxf(m, Elem<T>::get(x[i]));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+#pragma unroll 8
+  for (long long i = lane; i < n; i += 32) s += exp2_fast((Elem<T>::get(x[i]) - m) * c);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return {m, 0.f, s};
+}
+
+// A row's scalars, fetched a row ahead.
+template <typename T, int KIND>
+LZ_DEV void prepare_params(const LzLossArgs& a, const StreamPlan& p, const T* x, long long r, RowParams& out, TopView t,
+                           int* hash, float c) {
+  const int lane = threadIdx.x % 32;
+  if (KIND != LZ_LOSS_DISTILL) {
+    if (lane == 0) {
+      const long long y = load_id(a.ids, a.ids64, r);
+      out.token = y < a.vocab ? (int)y : -1;
+      out.xy = y < a.vocab ? Elem<T>::get(x[y]) : 0.f;
+      if (KIND == LZ_LOSS_POLICY) {
+        out.adv = a.advantages[r];
+        out.old_logp2 = (double)a.old_logp[r] * kLog2e;
+        out.ref_logp2 = a.ref_logp ? (double)a.ref_logp[r] * kLog2e : 0.0;
+        out.weight = (a.weights ? (double)a.weights[r] : 1.0) * a.work[0];
+      }
+    }
+    __syncwarp();
+    return;
+  }
+  float m = -INFINITY;
+  bool bad = false;
+  for (int k = lane; k < a.top; k += 32) {
+    const long long id = load_id(a.ids, a.ids64, r * a.top + k);
+    const float v = id < 0 ? -INFINITY : top_value(a, r, k);
+    const bool in = id >= 0 && id < a.vocab;
+    bad |= id >= a.vocab;
+    t.id[k] = in ? (int)id : -1;
+    t.z[k] = in ? Elem<T>::get(x[id]) : 0.f;
+    t.q[k] = v;
+    m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  bad = __any_sync(~0u, bad);
+  float s = 0.f;
+  for (int k = lane; k < a.top; k += 32) s += m == -INFINITY ? 0.f : expf(t.q[k] - m);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  const float inv = s > 0.f || s != s ? 1.f / s : 0.f;
+  const double logsum = log((double)s);
+  double q_logq = 0.0, q_z = 0.0, q_sum = 0.0;
+  for (int k = lane; k < a.top; k += 32) {
+    const float v = t.q[k], q = m == -INFINITY ? 0.f : expf(v - m) * inv;
+    t.q[k] = q;
+    t.share[k] = t.id[k] < 0 ? -1.f : q;
+    if (q != 0.f) {  // NaN counts
+      q_logq += (double)q * ((double)v - m - logsum);
+      q_z += (double)q * ((double)t.z[k] * (double)c);
+      q_sum += (double)q;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    q_logq += __shfl_xor_sync(~0u, q_logq, o);
+    q_z += __shfl_xor_sync(~0u, q_z, o);
+    q_sum += __shfl_xor_sync(~0u, q_sum, o);
+  }
+  // Does an id stand in the list twice? Then its first entry gets all shares.
+  for (int k = lane; k < p.hash; k += 32) hash[k] = -1;
+  __syncwarp();
+  bool twice = false;
+  for (int k = lane; k < a.top; k += 32) {
+    const int id = t.id[k];
+    if (id < 0) continue;
+    for (unsigned h = (unsigned)id * 2654435761u >> 7;; ++h) {  // ends: the table is twice the list
+      const int was = atomicCAS(hash + (h & (p.hash - 1)), -1, id);
+      twice |= was == id;
+      if (was == -1 || was == id) break;
+    }
+  }
+  if (__any_sync(~0u, twice)) {
+    for (int k = lane; k < a.top; k += 32) {
+      if (t.id[k] < 0) continue;
+      float q = t.q[k];
+      bool first = true;
+      for (int o = 0; o < a.top; ++o) {
+        if (t.id[o] != t.id[k] || o == k) continue;
+        first &= o > k;
+        q += t.q[o];
+      }
+      t.share[k] = first ? q : -1.f;
+    }
+  }
+  if (lane == 0) {
+    out.weight = (a.weights ? (double)a.weights[r] : 1.0) * a.work[0];
+    out.slope = bad ? NAN : m == -INFINITY ? 0.f : (float)-out.weight;
+    out.q_logq = q_logq, out.q_z = q_z, out.q_sum = q_sum;
+  }
+  __syncwarp();
+}
+
+constexpr int kBatch = 4;  // vectors a thread has in work at a time
+
+// Sum over a thread's elements of 2^(x c - ref). ref is not the running maximum:
+// it is taken from the first batch and moves only when a batch's maximum is more
+// than 2^16 above it, which fp32 has room for (2^16 times the vocabulary), so the
+// exponentials of a batch wait for no maximum and the branch is seldom taken.
+struct LazySum {
+  float ref, limit;  // in units of x c, of x; ref is -inf (and taken as 0) before the first batch
+  uint64_t neg_ref, sum[2];
+  LZ_DEV void init(float c) {
+    ref = -INFINITY, neg_ref = 0, sum[0] = sum[1] = 0;
+    limit = -3e38f / fmaxf(c, 1.f);  // below this x c is beyond 32 bits: such entries count nothing
+  }
+  LZ_DEV void raise(float m, float c) {
+    const float f = exp2_fast(ref - m * c);
+    sum[0] = mul2(sum[0], pair(f, f)), sum[1] = mul2(sum[1], pair(f, f));
+    ref = m * c, neg_ref = pair(-ref, -ref);
+    limit = m + 16.f / c;
+  }
+};
+
+template <typename T>
+LZ_DEV uint4 minus_infinity() {
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : Elem<T>::N == 8 && std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
+
+template <typename T, int U>
+LZ_DEV void batch_sum(const uint4* w, uint64_t c2, uint64_t neg_ref, uint64_t* out) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint64_t p[Elem<T>::N / 2];
+    unpack_pairs<T>(w[u], p);
+#pragma unroll
+    for (int i = 0; i < Elem<T>::N / 2; ++i) {
+      float lo, hi;
+      unpair(fma2(p[i], c2, neg_ref), lo, hi);
+      out[i % 2] = add2(out[i % 2], pair(exp2_fast(lo), exp2_fast(hi)));
+    }
+  }
+}
+
+template <typename T, int U>
+LZ_DEV void take_batch(LazySum& s, const uint4* w, float c) {
+  const uint64_t c2 = pair(c, c);
+  float m = vector_max<T>(w[0]);
+#pragma unroll
+  for (int u = 1; u < U; ++u) m = fmaxf(m, vector_max<T>(w[u]));
+  uint64_t part[2] = {0, 0};
+  batch_sum<T, U>(w, c2, s.neg_ref, part);
+  if (m > s.limit) {
+    s.raise(m, c);
+    part[0] = part[1] = 0;
+    batch_sum<T, U>(w, c2, s.neg_ref, part);
+  }
+  s.sum[0] = add2(s.sum[0], part[0]), s.sum[1] = add2(s.sum[1], part[1]);
+}
+
+template <typename T, int KIND, bool GRAD, int W>
+__global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_constant__ LzLossArgs a,
+                                                                 const __grid_constant__ StreamPlan plan) {
+  constexpr int N = Elem<T>::N, kTake = W * 32;
+  constexpr int kChunkVecs = kBatch / 2 * kTake, kChunk = 16 * kChunkVecs;
+  extern __shared__ __align__(128) char smem[];
+  StreamShared& sh = *reinterpret_cast<StreamShared*>(smem);
+  char* const lists = smem + sizeof(StreamShared);
+  char* const ring = lists + list_bytes(KIND, a.top, plan.hash);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const long long cluster = blockIdx.x / ranks, clusters = gridDim.x / ranks;
+  const float c = (float)(kLog2e * (double)a.inv_temperature);
+  volatile int* const failed = &sh.failed;
+  // Rows of this cluster: i = cluster, cluster + clusters, ... below `limit`, those that count first.
+  const long long limit = plan.ordered ? a.rows : min(a.rows, clusters);
+  const int active = plan.ordered ? *work_active(a) : 0;
+  auto row_at = [&](long long i, long long* r) {
+    if (i >= limit) return false;
+    *r = plan.ordered ? (long long)work_order(a)[i] : i;
+    return plan.ordered ? i < active : row_counts<KIND>(a, i);
+  };
+  auto head_at = [&](long long i) {
+    RowHead h;
+    long long r;
+    if (row_at(i, &r)) h = slice_of(row_of<T>(a, r), r, a.vocab, rank, ranks, kChunkVecs);
+    else h.row = -1;
+    return h;
+  };
+  if (tid == 0) {
+    for (int s = 0; s < plan.slots; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], W);
+    }
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(&sh.parts[k], W);
+      mbar_init(&sh.peers[k], ranks);
+      mbar_init(&sh.dense[k], 1);
+    }
+    fence_mbar_init();
+    *failed = 0;
+  }
+  if (tid >= (W + 1) * 32 && lane < 2) sh.heads[lane] = head_at(cluster + lane * clusters);
+  cluster_sync();
+
+  if (warp == W) {  // ---- streams the slices into the ring
+    if (lane == 0) {
+      uint32_t slot = 0, round = 0;
+      RowHead h = sh.heads[0];
+      for (long long i = cluster; h.row >= 0; i += clusters) {
+        const RowHead next = head_at(i + clusters);
+        const char* from = reinterpret_cast<const char*>(row_of<T>(a, h.row) + h.lead) + (size_t)h.first * 16;
+        for (int k = 0; k < h.chunks && !*failed; ++k) {
+          if (round) ring_wait<false>(&sh.empty[slot], (round - 1) & 1, failed);
+          if (*failed) break;
+          const int vecs = min(kChunkVecs, h.count - k * kChunkVecs);
+          bulk_g2s(ring + (size_t)slot * kChunk, from + (size_t)k * kChunk, vecs * 16, &sh.full[slot]);
+          if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
+        }
+        h = next;
+      }
+      if (*failed) {  // what is in flight lands before the CTA ends
+        for (uint32_t s = 0; s < (uint32_t)plan.slots; ++s)
+          if (round || s < slot) mbar_wait(&sh.full[s], (s < slot ? round : round - 1) & 1, 1u << 20);
+      }
+    }
+    __syncwarp();
+  } else if (warp < W) {  // ---- sums, then the dense gradient
+    uint32_t slot = 0, round = 0;      // where the sums are
+    uint32_t again = 0;                // where the gradient is
+    LazySum sum;
+    sum.init(c);
+    int done = 0;  // chunks of the row that are in `sum`
+    // Chunks [done, upto) of a row, two at a time.
+    auto take = [&](const RowHead& h, int upto) {
+      for (; done < upto; done += 2) {
+        uint4 w[kBatch];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          w[2 * b] = w[2 * b + 1] = minus_infinity<T>();
+          if (done + b < upto) {
+            ring_wait<false>(&sh.full[slot], round & 1, failed);
+            const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk);
+            const int vecs = h.count - (done + b) * kChunkVecs;
+            if (tid < vecs) w[2 * b] = v[tid];
+            if (tid + kTake < vecs) w[2 * b + 1] = v[tid + kTake];
+            if (!GRAD) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.empty[slot]);
+            }
+            if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
+          }
+        }
+        take_batch<T, kBatch>(sum, w, c);
+      }
+      done = min(done, upto);
+    };
+    uint32_t turn = 0;
+    for (;; ++turn) {
+      // The row's head is there, and its place in `warp_part` free, when the row two before it is done with.
+      const int k = turn & 1;
+      if (!GRAD && turn >= 2) ring_wait<false>(&sh.dense[k], ((turn - 2) >> 1) & 1, failed);
+      const RowHead h = sh.heads[turn & 3];
+      if (h.row < 0) break;
+      const long long single = rank == 0 && tid < 2 * N ? single_of<T>(h, tid, a.vocab) : -1;
+      float alone = 0.f;
+      if (single >= 0) alone = Elem<T>::get(row_of<T>(a, h.row)[single]);
+      take(h, h.chunks);
+      if (single >= 0) {
+        if (alone > sum.limit) sum.raise(alone, c);
+        float neg_ref, unused;
+        unpair(sum.neg_ref, neg_ref, unused);
+        sum.sum[0] = add2(sum.sum[0], pair(exp2_fast(fmaf(alone, c, neg_ref)), 0.f));
+      }
+      float s0, s1, s2, s3;
+      unpair(sum.sum[0], s0, s1), unpair(sum.sum[1], s2, s3);
+      float m = sum.ref, all = (s0 + s1) + (s2 + s3);
+      lanes_join(m, all, 32);
+      if (lane == 0) {
+        sh.warp_part[k][warp] = make_float2(m, all);
+        mbar_arrive(&sh.parts[k]);
+      }
+      sum.init(c);
+      done = 0;
+      if (!GRAD) continue;
+      const RowHead& next = sh.heads[(turn + 1) & 3];
+      if (next.row >= 0) take(next, min(plan.early, next.chunks));
+      ring_wait<false>(&sh.dense[k], (turn >> 1) & 1, failed);
+      const RowDense d = sh.row_dense[k];
+      T* out = static_cast<T*>(a.grad) + h.row * a.vocab;
+      const uint64_t c2 = pair(c, c), f2 = pair(d.f, d.f), off2 = pair(-d.ref, -d.ref);
+      for (int ch = 0; ch < h.chunks; ++ch) {
+        const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)again * kChunk);
+        uint4* o = reinterpret_cast<uint4*>(out + h.lead) + h.first + (long long)ch * kChunkVecs;
+        const int vecs = h.count - ch * kChunkVecs;
+        if (d.f == 0.f) {
+#pragma unroll
+          for (int j = tid; j < kChunkVecs; j += kTake)
+            if (j < vecs) st_cs_v4(o + j, make_uint4(0, 0, 0, 0));
+        } else if (d.base == 0.f) {
+          uint4 w[kBatch / 2];
+#pragma unroll
+          for (int u = 0; u < kBatch / 2; ++u)
+            if (tid + u * kTake < vecs) w[u] = v[tid + u * kTake];
+#pragma unroll
+          for (int u = 0; u < kBatch / 2; ++u) {
+            uint64_t p[N / 2];
+            float e[N];
+            unpack_pairs<T>(w[u], p);
+#pragma unroll
+            for (int q = 0; q < N / 2; ++q) {
+              float lo, hi;
+              unpair(fma2(p[q], c2, off2), lo, hi);
+              unpair(mul2(f2, pair(exp2_fast(lo), exp2_fast(hi))), e[2 * q], e[2 * q + 1]);
+            }
+            if (tid + u * kTake < vecs) st_cs_v4(o + tid + u * kTake, Elem<T>::pack(e));
+          }
+        } else {
+          for (int j = tid; j < min(vecs, kChunkVecs); j += kTake) {
+            float e[N];
+            Elem<T>::unpack(v[j], e);
+#pragma unroll
+            for (int q = 0; q < N; ++q) e[q] = d.f * exp2_fast((e[q] - d.base) * c);
+            st_cs_v4(o + j, Elem<T>::pack(e));
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[again]);
+        if (++again == (uint32_t)plan.slots) again = 0;
+      }
+      if (single >= 0)
+        out[single] = Elem<T>::put(d.f == 0.f ? 0.f : d.f * exp2_fast(fmaf(alone - d.base, c, -d.ref)));
+    }
+    __syncwarp();
+    if (GRAD) {
+      if (lane == 0) mbar_arrive(&sh.parts[turn & 1]);  // the last row is written
+      for (long long i = (plan.ordered ? active : 0) + cluster; i < limit; i += clusters) {
+        long long r;
+        if (row_at(i, &r)) continue;
+        T* out = static_cast<T*>(a.grad) + r * a.vocab;
+        const RowHead h = slice_of(out, r, a.vocab, rank, ranks, kChunkVecs);
+        uint4* o = reinterpret_cast<uint4*>(out + h.lead) + h.first;
+        for (int j = tid; j < h.count; j += kTake) st_cs_v4(o + j, make_uint4(0, 0, 0, 0));
+        const long long single = rank == 0 && tid < 2 * N ? single_of<T>(h, tid, a.vocab) : -1;
+        if (single >= 0) out[single] = Elem<T>::put(0.f);
+      }
+    }
+  } else {  // ---- joins the sums; the rows' scalars, outputs and sparse entries
+    auto view = [&](int k) {
+      float* f = reinterpret_cast<float*>(lists) + k * 4 * a.top;
+      return TopView{reinterpret_cast<int*>(f), f + a.top, f + 2 * a.top, f + 3 * a.top};
+    };
+    int* const hash = reinterpret_cast<int*>(lists) + 8 * a.top;
+    double loss = 0.0;
+    RowHead before = {-1};  // the row whose dense part is being written, its slope, token and sum
+    float before_slope = 0.f, before_xy = 0.f;
+    int before_token = -1;
+    RowSum before_n = {0.f, 0.f, 1.f};
+    auto sparse = [&](int k) {
+      if (!GRAD || before.row < 0 || before_slope == 0.f) return;
+      T* out = static_cast<T*>(a.grad) + before.row * a.vocab;
+      const long long lo = before.lead + (long long)before.first * N, hi = lo + (long long)before.count * N;
+      const long long tail = before.lead + (long long)before.vecs * N;
+      const float inv = 1.f / before_n.sum;
+      auto put = [&](int id, float z, float t) {
+        if (!((id >= lo && id < hi) || (rank == 0 && (id < before.lead || id >= tail)))) return;
+        const float p = exp2_fast(fmaf(z - before_n.base, c, -before_n.ref)) * inv;
+        out[id] = Elem<T>::put(before_slope * a.inv_temperature * (t - p));
+      };
+      if (KIND == LZ_LOSS_DISTILL) {
+        const TopView t = view(k);
+        for (int j = lane; j < a.top; j += 32)
+          if (!(t.share[j] < 0.f)) put(t.id[j], t.z[j], t.share[j]);
+      } else if (lane == 0 && before_token >= 0) {
+        put(before_token, before_xy, 1.f);
+      }
+    };
+    auto prepare = [&](const RowHead& h, int k) {
+      if (h.row >= 0) prepare_params<T, KIND>(a, plan, row_of<T>(a, h.row), h.row, sh.params, view(k), hash, c);
+    };
+    prepare(sh.heads[0], 0);
+    uint32_t turn = 0;
+    for (;; ++turn) {
+      const RowHead h = sh.heads[turn & 3];
+      if (h.row < 0) break;
+      const int k = turn & 1;
+      const RowHead later = head_at(cluster + (long long)(turn + 2) * clusters);
+      ring_wait<false>(&sh.parts[k], (turn >> 1) & 1, failed);
+      float2 v = sh.warp_part[k][lane % W];
+      lanes_join(v.x, v.y, W);
+      if (ranks > 1) {
+        if (lane < ranks) send_to_peer(&sh.peer_part[k][rank], v, &sh.peers[k], lane);
+        __syncwarp();
+        ring_wait<true>(&sh.peers[k], (turn >> 1) & 1, failed);
+        v = sh.peer_part[k][lane % ranks];
+        lanes_join(v.x, v.y, (int)ranks);
+      }
+      RowSum n = {0.f, v.x, v.y};
+      if (isinf(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
+      const RowParams& p = sh.params;
+      const Norm norm = n.norm();
+      const double logp2 = p.token < 0 ? (double)NAN : ((double)p.xy - (double)norm.base) * (double)c - norm.lse2;
+      PolicyOut o = {0.f, 0.f, false};
+      if (KIND == LZ_LOSS_POLICY) o = policy_out(a, p, logp2);
+      const float slope = KIND == LZ_LOSS_DISTILL ? p.slope : o.slope;
+      if (lane == 0) {
+        sh.row_dense[k] = {slope == 0.f ? 0.f : -slope * a.inv_temperature / n.sum, n.base, n.ref};
+        sh.heads[(turn + 2) & 3] = later;
+        mbar_arrive(&sh.dense[k]);
+      }
+      sparse(k ^ 1);
+      double kl = 0.0;
+      if (KIND == LZ_LOSS_DISTILL) {
+        kl = p.q_logq - kLn2 * (p.q_z - p.q_sum * norm.lse2);
+        if (norm.base != 0.f) {
+          const TopView t = view(k);
+          kl = 0.0;
+          for (int j = lane; j < a.top; j += 32)
+            if (t.q[j] != 0.f)
+              kl += (double)t.q[j] * (log((double)t.q[j]) -
+                                      (((double)t.z[j] - (double)norm.base) * (double)c - norm.lse2) * kLn2);
+#pragma unroll
+          for (int o2 = 16; o2; o2 >>= 1) kl += __shfl_xor_sync(~0u, kl, o2);
+        }
+        if (isnan(p.slope)) kl = NAN;
+      }
+      if (rank == 0 && lane == 0) {
+        double each = kl;
+        if (KIND != LZ_LOSS_DISTILL) a.logp[h.row] = (float)(logp2 * kLn2);
+        if (KIND == LZ_LOSS_POLICY) {
+          const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
+          each = -(double)p.adv * (o.clipped ? (p.adv > 0.f ? hi : lo) : (double)o.ratio);
+          if (a.ref_logp) {
+            const double d = (double)a.ref_logp[h.row] - logp2 * kLn2, e = expm1(d) - d;
+            a.kl[h.row] = (float)e;
+            each += (double)a.kl_coef * e;
+          }
+          a.clipped[h.row] = o.clipped;
+        }
+        if (KIND == LZ_LOSS_DISTILL) a.kl[h.row] = (float)kl;
+        if (KIND != LZ_LOSS_LOGP) loss += p.weight * each;
+        work_norm(a)[h.row] = make_double2(norm.base, norm.lse2);
+        work_slope(a)[h.row] = (double)slope;
+      }
+      before = h, before_n = n, before_slope = slope, before_xy = p.xy, before_token = p.token;
+      __syncwarp();
+      prepare(sh.heads[(turn + 1) & 3], k ^ 1);
+    }
+    if (GRAD) {
+      ring_wait<false>(&sh.parts[turn & 1], (turn >> 1) & 1, failed);
+      sparse((turn & 1) ^ 1);
+    }
+    if (rank == 0) {
+      long long r;
+      for (long long i = (plan.ordered ? active : 0) + cluster + lane * clusters; i < limit; i += 32 * clusters) {
+        if (row_at(i, &r)) continue;
+        if (KIND != LZ_LOSS_DISTILL) a.logp[r] = 0.f;
+        if (KIND == LZ_LOSS_DISTILL || (KIND == LZ_LOSS_POLICY && a.ref_logp)) a.kl[r] = 0.f;
+        if (KIND == LZ_LOSS_POLICY) a.clipped[r] = 0;
+        work_norm(a)[r] = make_double2(0.0, 0.0);
+        work_slope(a)[r] = 0.0;
+      }
+      if (*failed) {
+        loss = NAN;
+        for (long long i = cluster + lane * clusters; i < limit; i += 32 * clusters) {
+          row_at(i, &r);
+          if (KIND != LZ_LOSS_DISTILL) a.logp[r] = NAN;
+          if (KIND == LZ_LOSS_DISTILL || (KIND == LZ_LOSS_POLICY && a.ref_logp)) a.kl[r] = NAN;
+        }
+      }
+      if (KIND != LZ_LOSS_LOGP) {  // the cluster that is done last adds the losses up, in the clusters' order
+        int last = 0;
+        if (lane == 0) {
+          work_loss(a)[cluster] = loss;
+          __threadfence();
+          last = atomicAdd(work_ticket(a), 1u) == (unsigned)clusters - 1;
+        }
+        if (__shfl_sync(~0u, last, 0)) {
+          __threadfence();
+          double s = 0.0;
+          for (long long j = lane; j < clusters; j += 32) s += __ldcg(work_loss(a) + j);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+          if (lane == 0) *a.loss = (float)s;
+        }
+      }
+    }
+    __syncwarp();
+  }
+  cluster_sync();  // no CTA leaves while a peer may still write to it
 }
 
 // Preference loss of one pair a CTA: sums of its two sequences' log-probabilities
@@ -587,19 +1373,108 @@ int grid_for(int device, long long rows, int* grid) {
 
 size_t top_bytes(const LzLossArgs* a) { return a->kind == LZ_LOSS_DISTILL ? sizeof(Top) : 0; }
 
-template <typename T, int KIND>
-int launch_forward(const LzLossArgs* a, cudaStream_t s) {
-  if (KIND != LZ_LOSS_LOGP) {
-    head_kernel<<<1, kThreads, 0, s>>>(*a);
+// The stream kernel's launch for these arguments, or false where a CTA a row
+// does better or is the only way: rows that fit no cluster's shared memory,
+// rows and gradient rows at different offsets from a 16-byte border, small rows.
+struct StreamLaunch {
+  StreamPlan plan;
+  int clusters, ranks;
+  size_t smem;
+};
+
+constexpr int kStreamWarps = 16;
+constexpr int kChunk = 16 * kBatch / 2 * kStreamWarps * 32;  // bytes of a ring slot: half a batch of every thread
+constexpr int kSharedMax = 232448;
+constexpr int kMaxDevices = 64;
+
+template <typename T, int KIND, bool GRAD>
+int plan_stream(const LzLossArgs* a, StreamLaunch* l, bool* fits) {
+  *fits = false;
+  const long long row = a->vocab * (long long)sizeof(T);
+  if (row < 16384 || a->rows > INT32_MAX) return LZE_OK;
+  if (GRAD && ((((uintptr_t)a->logits ^ (uintptr_t)a->grad) % 16) ||
+               (a->inner < a->rows && (a->outer_stride * (long long)sizeof(T) - a->inner * row) % 16) ||
+               (a->inner > 1 && (a->inner_stride * (long long)sizeof(T) - row) % 16)))
+    return LZE_OK;
+  int hash = 0;
+  if (KIND == LZ_LOSS_DISTILL)
+    for (hash = 32; hash < 2 * a->top;) hash *= 2;
+  const int fixed = (int)sizeof(StreamShared) + list_bytes(KIND, a->top, hash);
+  const int slots = (kSharedMax - fixed) / kChunk < kMaxSlots ? (kSharedMax - fixed) / kChunk : kMaxSlots;
+  auto kernel = stream_kernel<T, KIND, GRAD, kStreamWarps>;
+  static std::atomic<bool> known[kMaxDevices];
+  static std::atomic<int> resident[kMaxDevices][4];
+  if (a->device < 0 || a->device >= kMaxDevices) return LZE_OK;
+  if (!known[a->device].load(std::memory_order_acquire)) {
+    LZ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
+    for (int k = 0; k < 4; ++k) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute at[1] = {};
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim = {1u << k, 1, 1};
+      cfg.gridDim = dim3(148 * 8), cfg.blockDim = dim3((kStreamWarps + 2) * 32), cfg.dynamicSmemBytes = kSharedMax;
+      cfg.attrs = at, cfg.numAttrs = 1;
+      int g = 0;
+      LZ_CUDA_TRY(cudaOccupancyMaxActiveClusters(&g, kernel, &cfg));
+      resident[a->device][k].store(g, std::memory_order_relaxed);
+    }
+    known[a->device].store(true, std::memory_order_release);
+  }
+  double best = 0.0;
+  int chunks = 0;
+  for (int k = 0; k < 4; ++k) {
+    const int ranks = 1 << k, g = resident[a->device][k].load(std::memory_order_relaxed);
+    const long long slice = (row + ranks - 1) / ranks;
+    if (g < 1 || (GRAD && (slice + 16 + kChunk - 1) / kChunk > slots)) continue;
+    const double cost = (double)((a->rows + g - 1) / g) * ((double)slice * (GRAD ? 2 : 1) + 50e3);
+    if (best != 0.0 && cost >= best) continue;
+    best = cost;
+    l->ranks = ranks;
+    l->clusters = (int)(a->rows < g ? a->rows : g);
+    chunks = (int)((slice + 16 + kChunk - 1) / kChunk);
+  }
+  if (best == 0.0) return LZE_OK;
+  l->plan = {slots, (slots - chunks) / 2 * 2, a->rows > l->clusters, hash};
+  l->smem = fixed + (size_t)slots * kChunk;
+  *fits = true;
+  return LZE_OK;
+}
+
+template <typename T, int KIND, bool GRAD>
+int launch_stream(const LzLossArgs* a, const StreamLaunch& l, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)l.ranks, 1, 1};
+  cfg.gridDim = dim3(l.clusters * l.ranks), cfg.blockDim = dim3((kStreamWarps + 2) * 32);
+  cfg.dynamicSmemBytes = l.smem, cfg.stream = s, cfg.attrs = at, cfg.numAttrs = 1;
+  LZ_CUDA_TRY(cudaLaunchKernelEx(&cfg, stream_kernel<T, KIND, GRAD, kStreamWarps>, *a, l.plan));
+  return LZE_OK;
+}
+
+template <typename T, int KIND, bool GRAD>
+int launch_forward_as(const LzLossArgs* a, cudaStream_t s) {
+  StreamLaunch l = {};
+  bool fits = false;
+  if (a->rows)
+    if (const int rc = plan_stream<T, KIND, GRAD>(a, &l, &fits)) return rc;
+  if (KIND != LZ_LOSS_LOGP || l.plan.ordered) {
+    head_kernel<KIND><<<1, kThreads, 0, s>>>(*a, l.plan.ordered);
     LZ_CUDA_TRY(cudaGetLastError());
   }
   if (!a->rows) return LZE_OK;
+  if (fits) return launch_stream<T, KIND, GRAD>(a, l, s);
   int grid = 0;
   if (const int rc = grid_for(a->device, a->rows, &grid)) return rc;
-  if (a->grad) forward_kernel<T, KIND, true><<<grid, kThreads, top_bytes(a), s>>>(*a);
-  else forward_kernel<T, KIND, false><<<grid, kThreads, top_bytes(a), s>>>(*a);
+  forward_kernel<T, KIND, GRAD><<<grid, kThreads, top_bytes(a), s>>>(*a);
   LZ_CUDA_TRY(cudaGetLastError());
   return LZE_OK;
+}
+
+template <typename T, int KIND>
+int launch_forward(const LzLossArgs* a, cudaStream_t s) {
+  if constexpr (KIND == LZ_LOSS_LOGP) return launch_forward_as<T, KIND, false>(a, s);
+  else return a->grad ? launch_forward_as<T, KIND, true>(a, s) : launch_forward_as<T, KIND, false>(a, s);
 }
 
 template <typename T, int KIND>

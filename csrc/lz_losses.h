@@ -10,8 +10,10 @@
 
 #define LZ_LOSS_MAX_TOP 1024
 
-// Doubles in front of the per-row parts of `work`: 1 / denominator, ticket.
+// Doubles in front of the per-row parts of `work` (1 / denominator; ticket and
+// number of rows that count) and per row.
 #define LZ_LOSS_WORK_HEAD 2
+#define LZ_LOSS_WORK_ROW 5
 
 #ifdef __cplusplus
 extern "C" {
@@ -37,8 +39,9 @@ struct LzLossArgs {
   float* logp;           // [rows] (LOGP, POLICY)
   float* kl;             // [rows] (POLICY with ref_logp, DISTILL)
   unsigned char* clipped;  // [rows] (POLICY)
-  // [HEAD + 4 rows], 16-byte aligned: head, then per row its normaliser (two
-  // doubles), the slope of the loss in its log-probability, its loss
+  // [HEAD + ROW rows], 16-byte aligned: head, then per row its normaliser (two
+  // doubles), the slope of the loss in its log-probability, its loss, and its
+  // place in the order in which rows are taken (int)
   double* work;
   double denom;          // denominator; < 0: the sum of the weights
   float inv_temperature, clip_low, clip_high, kl_coef;

@@ -40,8 +40,9 @@ from ..utils.dtypes import LZ_BF16, LZ_F16, LZ_F32
 from ..utils.trace import traced
 
 LOGP, POLICY, DISTILL = 0, 1, 2
+_NAMES = ("token log-probabilities", "policy loss", "distillation loss")
 MAX_TOP = 1024
-_HEAD, _PER_ROW = 2, 4  # doubles of the workspace (csrc/lz_losses.h)
+_HEAD, _PER_ROW = 2, 5  # doubles of the workspace (csrc/lz_losses.h)
 _DTYPES = {torch.float32: LZ_F32, torch.float16: LZ_F16, torch.bfloat16: LZ_BF16}
 _IDS = (torch.int64, torch.int32)
 
@@ -105,7 +106,7 @@ def _check_logits(what: str, logits: torch.Tensor) -> None:
 def _check_ids(what: str, name: str, ids: torch.Tensor, shape, device) -> torch.Tensor:
     if ids.dtype not in _IDS:
         raise TypeError(f"{what}: {name} are {ids.dtype}; expected int64 or int32")
-    if tuple(ids.shape) != tuple(shape):
+    if ids.shape != shape:
         raise ValueError(f"{what}: {name} have shape {tuple(ids.shape)}; expected {tuple(shape)}")
     if ids.device != device:
         raise ValueError(f"{what}: {name} are on {ids.device}, the logits on {device}")
@@ -118,13 +119,13 @@ def _check_rows(what: str, name: str, t: torch.Tensor | None, shape, device, any
         return None
     if not (t.is_floating_point() or any_type) or t.is_complex():
         raise TypeError(f"{what}: {name} is {t.dtype}; expected a floating-point type")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}; expected {tuple(shape)}")
     if t.device != device:
         raise ValueError(f"{what}: {name} is on {t.device}, the logits on {device}")
     if t.requires_grad:
         raise ValueError(f"{what}: {name} requires a gradient, and this loss gives none to it; detach it")
-    return t.to(torch.float32).contiguous()
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _check_number(what: str, name: str, v, low: float, high: float = math.inf, open_low: bool = False) -> float:
@@ -155,6 +156,9 @@ def _check_denom(what: str, denom, device):
 
 
 # ---- native calls ---------------------------------------------------------------------------------------
+#
+# Small calls are bound by what runs on the host, so the arguments are built in one
+# go, once per call, and the backward pass takes the forward pass's.
 
 
 def _ptr(t: torch.Tensor | None):
@@ -162,200 +166,195 @@ def _ptr(t: torch.Tensor | None):
 
 
 def _rows_of(x: torch.Tensor):
-    """(tensor, rows, inner, outer stride, inner stride): row r starts at
+    """(tensor, outer stride, inner stride, inner, rows): row r starts at
     (r // inner) * outer stride + (r % inner) * inner stride. Copies only where
     two strides and a contiguous vocabulary cannot say it."""
+    v = x.shape[-1]
+    if x.is_contiguous():
+        rows = x.numel() // v
+        return x, 0, v, max(1, rows), rows
     lead = x.shape[:-1]
-    rows = math.prod(lead)
-    if x.stride(-1) != 1 and x.shape[-1] > 1 or len(lead) > 2:
-        x = x.contiguous()
-    if len(lead) > 2 or x.is_contiguous():
-        return x, rows, max(1, rows), 0, x.shape[-1]
+    if x.stride(-1) != 1 and v > 1 or len(lead) > 2:
+        return _rows_of(x.contiguous())
     if len(lead) == 2:
-        return x, rows, max(1, lead[1]), x.stride(0), x.stride(1)
-    return x, rows, max(1, rows), 0, x.stride(0) if lead else 0
+        return x, x.stride(0), x.stride(1), max(1, lead[1]), lead[0] * lead[1]
+    return x, 0, x.stride(0) if lead else 0, max(1, math.prod(lead)), math.prod(lead)
 
 
-def _args(kind: int, logits: torch.Tensor, ids: torch.Tensor, work: torch.Tensor, temperature: float) -> _LossArgs:
-    x, rows, inner, outer_stride, inner_stride = _rows_of(logits)
-    a = _LossArgs(kind=kind, logits=x.data_ptr(), rows=rows, inner=inner, outer_stride=outer_stride,
-                  inner_stride=inner_stride, vocab=x.shape[-1], ids=ids.data_ptr(), ids64=ids.dtype == torch.int64,
-                  work=work.data_ptr(), inv_temperature=1.0 / temperature, dtype=_DTYPES[x.dtype], device=x.device.index)
-    a.copied = x  # alive as long as the arguments are
-    return a
+_lib = None
 
 
-def _launch(fn: str, a, device, what: str) -> None:
-    stream = torch.cuda.current_stream(device).cuda_stream
-    _native.check(getattr(_native.cuda(), fn)(C.byref(a), stream), what)
+def _launch(fn: str, a, what: str) -> None:
+    global _lib
+    if _lib is None:
+        _lib = _native.cuda()
+    rc = getattr(_lib, fn)(C.byref(a), torch._C._cuda_getCurrentRawStream(a.device))
+    if rc:
+        _native.check(rc, what)
 
 
-def _work(logits: torch.Tensor) -> torch.Tensor:
-    rows = math.prod(logits.shape[:-1])
-    return torch.empty(_HEAD + _PER_ROW * rows, dtype=torch.float64, device=logits.device)
+def _start(kind: int, logits: torch.Tensor, ids: torch.Tensor, temperature: float, denom=None, grad=None, teacher=None,
+           rows=(None, None, None, None), out=(None, None, None, None), numbers=(0.0, 0.0, 0.0)):
+    """Runs the forward pass; returns its arguments, the logits as they were read and the workspace."""
+    x, outer_stride, inner_stride, inner, n = _rows_of(logits)
+    work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=x.device)
+    old, adv, ref, weights = rows
+    loss, logp, kl, clipped = out
+    on_device = isinstance(denom, torch.Tensor)
+    a = _LossArgs(
+        x.data_ptr(), outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(grad), ids.data_ptr(), _ptr(teacher),
+        _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights), denom.data_ptr() if on_device else None, None, None, _ptr(loss),
+        _ptr(logp), _ptr(kl), _ptr(clipped), work.data_ptr(), -1.0 if denom is None or on_device else denom,
+        1.0 / temperature, *numbers, kind, _DTYPES[x.dtype], ids.dtype is torch.int64,
+        ids.shape[-1] if teacher is not None else 0, _DTYPES[teacher.dtype] if teacher is not None else 0,
+        x.device.index, 0)
+    _launch("lz_loss_forward", a, _NAMES[kind])
+    return a, x, work
 
 
-def _grad_buffer(logits: torch.Tensor) -> torch.Tensor:
-    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-
-
-def _set_denom(a: _LossArgs, denom) -> None:
-    if isinstance(denom, torch.Tensor):
-        a.denom_ptr = denom.data_ptr()
-    else:
-        a.denom = -1.0 if denom is None else denom
-
-
-def _logprobs_forward(logits, tokens, temperature):
-    logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
-    work = _work(logits)
-    a = _args(LOGP, logits, tokens, work, temperature)
-    a.logp = logp.data_ptr()
-    _launch("lz_loss_forward", a, logits.device, "token log-probabilities")
-    return logp, work
-
-
-def _logprobs_backward(logits, tokens, work, temperature, row_upstream, upstream=None):
-    grad = _grad_buffer(logits)
-    a = _args(LOGP, logits, tokens, work, temperature)
-    a.grad, a.row_upstream, a.upstream, a.fresh = grad.data_ptr(), row_upstream.data_ptr(), _ptr(upstream), 1
-    _launch("lz_loss_backward", a, logits.device, "token log-probabilities, backward")
+def _finish(a: _LossArgs, x: torch.Tensor, ids: torch.Tensor, work: torch.Tensor, shape, grad=None, upstream=None,
+            row_upstream=None, teacher=None) -> torch.Tensor:
+    """Runs the backward pass with the forward pass's arguments `a`; `grad` is what that left, if it did."""
+    if x.data_ptr() != a.logits:  # a saved tensor that came back from elsewhere
+        x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(x)
+    a.logits, a.ids, a.work, a.fresh = x.data_ptr(), ids.data_ptr(), work.data_ptr(), grad is None
+    if teacher is not None:
+        a.teacher = teacher.data_ptr()
+    if grad is None:
+        grad = torch.empty(shape, dtype=x.dtype, device=x.device)
+    a.grad, a.upstream, a.row_upstream = grad.data_ptr(), _ptr(upstream), _ptr(row_upstream)
+    _launch("lz_loss_backward", a, _NAMES[a.kind])
     return grad
 
 
-class _TokenLogprobs(torch.autograd.Function):
+def _grad_like(logits: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _fp32(g: torch.Tensor) -> torch.Tensor:
+    return g if g.dtype is torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
+
+
+class _Loss(torch.autograd.Function):
+    """What the three losses and the log-probabilities share: the backward pass
+    is not differentiable itself, and says so where a graph of it is recorded."""
+
+    @classmethod
+    def backward(cls, ctx, g, *_):
+        if g is None:
+            return (None,) * ctx.inputs
+        if torch.is_grad_enabled():
+            return cls._recorded(ctx, g)
+        return (cls.gradient(ctx, g), *(None,) * (ctx.inputs - 1))
+
+    @classmethod
+    def _recorded(cls, ctx, g):
+        def gradient(ctx, g):
+            return cls.gradient(ctx, g)
+
+        return (torch.autograd.function.once_differentiable(gradient)(ctx, g), *(None,) * (ctx.inputs - 1))
+
+
+def _scalar_gradient(ctx, g):
+    """The gradient that the forward pass left, for upstream `g`. It is handed
+    out once: a second pass over a retained graph writes into memory of its own."""
+    x, ids, work, *teacher = ctx.saved_tensors
+    grad, ctx.grad = ctx.grad, None
+    return _finish(ctx.args, x, ids, work, ctx.shape, grad, _fp32(g), None, *teacher)
+
+
+def _run_token_logprobs(logits, tokens, temperature):
+    logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+    return logp, *_start(LOGP, logits, tokens, temperature, out=(None, logp, None, None))
+
+
+class _TokenLogprobs(_Loss):
     @staticmethod
     def forward(ctx, logits, tokens, temperature):
-        logp, work = _logprobs_forward(logits, tokens, temperature)
-        ctx.save_for_backward(logits, tokens, work)
-        ctx.temperature = temperature
+        logp, ctx.args, x, work = _run_token_logprobs(logits, tokens, temperature)
+        ctx.save_for_backward(x, tokens, work)
+        ctx.shape, ctx.inputs = logits.shape, 3
         return logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        logits, tokens, work = ctx.saved_tensors
-        g = g.to(torch.float32).contiguous()
-        return _logprobs_backward(logits, tokens, work, ctx.temperature, g), None, None
+    def gradient(ctx, g):
+        x, ids, work = ctx.saved_tensors
+        return _finish(ctx.args, x, ids, work, ctx.shape, row_upstream=_fp32(g))
 
 
-def _policy_forward(logits, tokens, rows, p, grad):
+def _run_policy(logits, tokens, rows, p, grad=None):
     """rows: old_logp, advantages, ref_logp, weights; p: the loss's numbers."""
-    old, adv, ref, weights = rows
-    dev = logits.device
-    work = _work(logits)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    kl = None if ref is None else torch.empty_like(logp)
-    clipped = torch.empty(tokens.shape, dtype=torch.bool, device=dev)
-    a = _args(POLICY, logits, tokens, work, p["temperature"])
-    a.old_logp, a.advantages, a.ref_logp, a.weights = _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights)
-    a.loss, a.logp, a.kl, a.clipped, a.grad = _ptr(loss), _ptr(logp), _ptr(kl), _ptr(clipped), _ptr(grad)
-    a.clip_low, a.clip_high, a.kl_coef = p["clip_low"], p["clip_high"], p["kl_coef"]
-    _set_denom(a, p["denom"])
-    _launch("lz_loss_forward", a, dev, "policy loss")
-    return loss, logp, kl, clipped, work
+    old = rows[0]  # contiguous, fp32, of the tokens' shape
+    out = (old.new_empty(()), torch.empty_like(old), None if rows[2] is None else torch.empty_like(old),
+           torch.empty_like(old, dtype=torch.bool))
+    return out, *_start(POLICY, logits, tokens, p["temperature"], p["denom"], grad, None, rows, out,
+                        (p["clip_low"], p["clip_high"], p["kl_coef"]))
 
 
-def _distill_forward(logits, ids, teacher, weights, p, grad):
-    dev = logits.device
-    work = _work(logits)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    a = _args(DISTILL, logits, ids, work, p["temperature"])
-    a.teacher, a.teacher_dtype, a.top, a.weights = _ptr(teacher), _DTYPES[teacher.dtype], ids.shape[-1], _ptr(weights)
-    a.loss, a.kl, a.grad = _ptr(loss), _ptr(kl), _ptr(grad)
-    _set_denom(a, p["denom"])
-    _launch("lz_loss_forward", a, dev, "distillation loss")
-    return loss, kl, work
-
-
-def _scalar_backward(ctx, kind, g, logits, ids, work, teacher=None):
-    """The gradient that the forward pass left, for upstream `g`. It is handed
-    out once: a second pass over a retained graph writes into memory of its own."""
-    grad, ctx.grad = ctx.grad, None
-    a = _args(kind, logits, ids, work, ctx.p["temperature"])
-    a.fresh = grad is None
-    if grad is None:
-        grad = _grad_buffer(logits)
-    if teacher is not None:
-        a.teacher, a.teacher_dtype, a.top = _ptr(teacher), _DTYPES[teacher.dtype], ids.shape[-1]
-    g = g.to(torch.float32)
-    a.grad, a.upstream = grad.data_ptr(), g.data_ptr()
-    _launch("lz_loss_backward", a, logits.device, "loss, backward")
-    return grad
-
-
-class _PolicyLoss(torch.autograd.Function):
+class _PolicyLoss(_Loss):
     @staticmethod
     def forward(ctx, logits, tokens, rows, p):
-        ctx.grad, ctx.p = _grad_buffer(logits), p
-        loss, logp, kl, clipped, work = _policy_forward(logits, tokens, rows, p, ctx.grad)
-        ctx.save_for_backward(logits, tokens, work)
-        ctx.mark_non_differentiable(*(t for t in (logp, kl, clipped) if t is not None))
+        ctx.grad = _grad_like(logits)
+        out, ctx.args, x, work = _run_policy(logits, tokens, rows, p, ctx.grad)
+        ctx.save_for_backward(x, tokens, work)
+        ctx.mark_non_differentiable(*(t for t in out[1:] if t is not None))
         ctx.set_materialize_grads(False)
-        return loss, logp, kl, clipped
+        ctx.shape, ctx.inputs = logits.shape, 4
+        return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
-            return None, None, None, None
-        return _scalar_backward(ctx, POLICY, g, *ctx.saved_tensors), None, None, None
+    gradient = staticmethod(_scalar_gradient)
 
 
-class _DistillLoss(torch.autograd.Function):
+def _run_distill(logits, ids, teacher, weights, p, grad=None):
+    dev = logits.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    return (loss, kl), *_start(DISTILL, logits, ids, p["temperature"], p["denom"], grad, teacher,
+                               (None, None, None, weights), (loss, None, kl, None))
+
+
+class _DistillLoss(_Loss):
     @staticmethod
     def forward(ctx, logits, ids, teacher, weights, p):
-        ctx.grad, ctx.p = _grad_buffer(logits), p
-        loss, kl, work = _distill_forward(logits, ids, teacher, weights, p, ctx.grad)
-        ctx.save_for_backward(logits, ids, work, teacher)
-        ctx.mark_non_differentiable(kl)
+        ctx.grad = _grad_like(logits)
+        out, ctx.args, x, work = _run_distill(logits, ids, teacher, weights, p, ctx.grad)
+        ctx.save_for_backward(x, ids, work, teacher)
+        ctx.mark_non_differentiable(out[1])
         ctx.set_materialize_grads(False)
-        return loss, kl
+        ctx.shape, ctx.inputs = logits.shape, 5
+        return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
-            return None, None, None, None, None
-        return _scalar_backward(ctx, DISTILL, g, *ctx.saved_tensors), None, None, None, None
+    gradient = staticmethod(_scalar_gradient)
 
 
-def _preference_forward(logits, tokens, ref, offsets, p):
-    logp, work = _logprobs_forward(logits, tokens, p["temperature"])
+def _run_preference(logits, tokens, ref, offsets, p):
+    logp, args, x, work = _run_token_logprobs(logits, tokens, p["temperature"])
     dev, pairs, rows = logits.device, p["pairs"], tokens.numel()
     loss = torch.empty((), dtype=torch.float32, device=dev)
     rewards = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
     pair_work = torch.empty(1 + pairs + (rows + 1) // 2, dtype=torch.float64, device=dev)
-    a = _PairArgs(logp=_ptr(logp), ids=_ptr(tokens), offsets=_ptr(offsets), ref_logp=_ptr(ref), loss=_ptr(loss),
-                  rewards=_ptr(rewards), work=_ptr(pair_work), rows=rows, pairs=pairs, length=p["length"],
-                  beta=p["beta"], smoothing=p["label_smoothing"], normalized=p["length_normalized"],
-                  ids64=tokens.dtype == torch.int64, offsets64=offsets is not None and offsets.dtype == torch.int64,
-                  device=dev.index)
-    _launch("lz_loss_pairs", a, dev, "preference loss")
-    slope = pair_work[1 + pairs:].view(torch.float32)
-    return loss, rewards, work, slope
+    a = _PairArgs(logp.data_ptr(), tokens.data_ptr(), _ptr(offsets), _ptr(ref), loss.data_ptr(), rewards.data_ptr(),
+                  pair_work.data_ptr(), rows, pairs, p["length"], p["beta"], p["label_smoothing"], p["length_normalized"],
+                  tokens.dtype is torch.int64, offsets is not None and offsets.dtype is torch.int64, dev.index)
+    _launch("lz_loss_pairs", a, "preference loss")
+    return loss, rewards, args, x, work, pair_work
 
 
-class _PreferenceLoss(torch.autograd.Function):
+class _PreferenceLoss(_Loss):
     @staticmethod
     def forward(ctx, logits, tokens, ref, offsets, p):
-        loss, rewards, work, slope = _preference_forward(logits, tokens, ref, offsets, p)
-        ctx.save_for_backward(logits, tokens, work, slope)
-        ctx.temperature = p["temperature"]
+        loss, rewards, ctx.args, x, work, pair_work = _run_preference(logits, tokens, ref, offsets, p)
+        ctx.save_for_backward(x, tokens, work, pair_work)
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
+        ctx.shape, ctx.inputs, ctx.pairs = logits.shape, 5, p["pairs"]
         return loss, rewards
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
-            return None, None, None, None, None
-        logits, tokens, work, slope = ctx.saved_tensors
-        g = g.to(torch.float32)
-        return _logprobs_backward(logits, tokens, work, ctx.temperature, slope, g), None, None, None, None
+    def gradient(ctx, g):
+        x, tokens, work, pair_work = ctx.saved_tensors
+        slope = pair_work[1 + ctx.pairs:].view(torch.float32)
+        return _finish(ctx.args, x, tokens, work, ctx.shape, upstream=_fp32(g), row_upstream=slope)
 
 
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------
@@ -453,7 +452,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
         return _cpu_token_logprobs(logits, tokens, temperature)
     if _needs_grad(logits):
         return _TokenLogprobs.apply(logits, tokens, temperature)
-    return _logprobs_forward(logits, tokens, temperature)[0]
+    return _run_token_logprobs(logits, tokens, temperature)[0]
 
 
 @traced("policy_loss")
@@ -490,7 +489,7 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
         return PolicyLoss(*_cpu_policy_loss(logits, tokens, rows, p))
     if _needs_grad(logits):
         return PolicyLoss(*_PolicyLoss.apply(logits, tokens, rows, p))
-    return PolicyLoss(*_policy_forward(logits, tokens, rows, p, None)[:4])
+    return PolicyLoss(*_run_policy(logits, tokens, rows, p)[0])
 
 
 @traced("preference_loss")
@@ -533,7 +532,7 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, *, ref_logp: tor
     elif _needs_grad(logits):
         loss, rewards = _PreferenceLoss.apply(logits, tokens, ref, cu_seqlens, p)
     else:
-        loss, rewards = _preference_forward(logits, tokens, ref, cu_seqlens, p)[:2]
+        loss, rewards = _run_preference(logits, tokens, ref, cu_seqlens, p)[:2]
     return PreferenceLoss(loss, rewards[:p["pairs"]], rewards[p["pairs"]:])
 
 
@@ -571,4 +570,4 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
         return DistillLoss(*_cpu_distill_loss(logits, ids, teacher, weights, p))
     if _needs_grad(logits):
         return DistillLoss(*_DistillLoss.apply(logits, ids, teacher, weights, p))
-    return DistillLoss(*_distill_forward(logits, ids, teacher, weights, p, None)[:2])
+    return DistillLoss(*_run_distill(logits, ids, teacher, weights, p)[0])
