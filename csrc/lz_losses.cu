@@ -241,7 +241,8 @@ template <typename T>
 LZ_DEV void row_dense(const T* x, T* out, long long n, double slope, float inv_t, const Norm& norm, float c) {
   constexpr int N = Elem<T>::N;
   const float l = (float)norm.lse2;
-  const float a = slope == 0.0 ? 0.f : (float)(-slope * inv_t * exp2((double)l - norm.lse2));
+  const double left = (double)l - norm.lse2;  // at most half a step of l: 2^left is 1 + left ln 2
+  const float a = slope == 0.0 ? 0.f : (float)(-slope * inv_t * (1.0 + left * kLn2));
   if (a == 0.f) {
     const Split<T> sp(out, n);
     uint4* v = reinterpret_cast<uint4*>(out + sp.lead);
@@ -260,13 +261,20 @@ LZ_DEV void row_dense(const T* x, T* out, long long n, double slope, float inv_t
   const Split<T> sp(x, n);
   const uint4* v = reinterpret_cast<const uint4*>(x + sp.lead);
   uint4* o = reinterpret_cast<uint4*>(out + sp.lead);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < sp.vecs; i += kThreads) {
-    float f[N];
-    Elem<T>::unpack(__ldg(v + i), f);
+  constexpr int U = 4;
+  for (int i = threadIdx.x; i < sp.vecs; i += U * kThreads) {
+    uint4 w[U];
 #pragma unroll
-    for (int k = 0; k < N; ++k) f[k] = a * exp2_fast(fmaf(f[k], c, -l));
-    st_cs_v4(o + i, Elem<T>::pack(f));
+    for (int u = 0; u < U; ++u)
+      if (i + u * kThreads < sp.vecs) w[u] = __ldg(v + i + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[N];
+      Elem<T>::unpack(w[u], f);
+#pragma unroll
+      for (int k = 0; k < N; ++k) f[k] = a * exp2_fast(fmaf(f[k], c, -l));
+      if (i + u * kThreads < sp.vecs) st_cs_v4(o + i + u * kThreads, Elem<T>::pack(f));
+    }
   }
   const long long tail = sp.lead + (long long)sp.vecs * N;
   const int singles = sp.lead + (int)(n - tail);
@@ -528,8 +536,18 @@ __global__ void __launch_bounds__(kThreads) head_kernel(const __grid_constant__ 
   if (threadIdx.x == 0) *work_active(a) = front;
 }
 
-// The gradient from the rows' saved sums and slopes. POLICY and DISTILL: where
-// `grad` holds the gradient for upstream 1 and the upstream is 1, it stands.
+// A row's slope for the given upstream.
+template <int KIND>
+LZ_DEV double row_slope_for(const LzLossArgs& a, long long r, long long y, float up) {
+  if (y >= a.vocab) return NAN;
+  if (KIND == LZ_LOSS_LOGP) return y < 0 ? 0.0 : (double)up * (double)a.row_upstream[r];
+  const double slope = work_slope(a)[r];
+  return slope == 0.0 ? 0.0 : (double)up * slope;
+}
+
+// The gradient from the rows' saved sums and slopes, a CTA a row. POLICY and
+// DISTILL: where `grad` holds the gradient for upstream 1 and the upstream is 1,
+// it stands.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ LzLossArgs a) {
   extern __shared__ char dynamic[];
@@ -541,10 +559,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
     T* out = static_cast<T*>(a.grad) + r * a.vocab;
     const Norm n = {(float)work_norm(a)[r].x, work_norm(a)[r].y};
     const long long y = KIND == LZ_LOSS_DISTILL ? 0 : load_id(a.ids, a.ids64, r);
-    double slope = (double)up;
-    if (KIND == LZ_LOSS_LOGP) slope = y < 0 ? 0.0 : slope * (double)a.row_upstream[r];
-    else slope = work_slope(a)[r] == 0.0 ? 0.0 : slope * work_slope(a)[r];
-    if (y >= a.vocab) slope = NAN;
+    const double slope = row_slope_for<KIND>(a, r, y, up);
     Top* top = reinterpret_cast<Top*>(dynamic);
     if (KIND == LZ_LOSS_DISTILL && slope != 0.0) {
       float tmax;
@@ -577,13 +592,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 
 constexpr int kMaxSlots = 64;
 constexpr int kMaxCluster = 8;
+constexpr int kSmallList = 128;  // teacher's lists up to here look for equal ids entry by entry, longer ones by a hash table
 constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of every wait
 
 struct StreamPlan {
   int slots;    // of the ring, a chunk each
   int early;    // chunks of the next row taken before this one's gradient
   int ordered;  // rows by work_order; otherwise one row a cluster
-  int hash;     // entries of the hash table of DISTILL, a power of two
+  int hash;     // entries of the hash table of DISTILL, a power of two; 0 where the list is short
 };
 
 struct RowParams {
@@ -619,12 +635,12 @@ __host__ __device__ inline int list_bytes(int kind, int top, int hash) {
 
 struct alignas(128) StreamShared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
-  uint64_t parts[2], peers[2], dense[2];  // of every other row
+  uint64_t parts[2], peers[2], dense[2], ready[2], used[2];  // of every other row
   float2 warp_part[2][16];
   float2 peer_part[2][kMaxCluster];
   RowHead heads[4];
   RowDense row_dense[2];
-  RowParams params;
+  RowParams params[2];
   int failed;
 };
 
@@ -644,49 +660,74 @@ LZ_DEV void cluster_sync() {
 LZ_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.shared::cta.b64 t, [%0];\n\t}" ::"r"(smem_addr(bar)) : "memory");
 }
-// Stores v at `slot` of CTA `rank`'s shared memory and arrives at its `bar`.
+// Sends v to `slot` of CTA `rank`'s shared memory; its 8 bytes count there on
+// `bar`. (A remote arrive with release semantics would first wait for this
+// thread's outputs to reach global memory.)
 LZ_DEV void send_to_peer(float2* slot, float2 v, uint64_t* bar, uint32_t rank) {
   asm volatile(
       "{\n\t.reg .b32 s, b;\n\t"
       "mapa.shared::cluster.u32 s, %0, %2;\n\t"
       "mapa.shared::cluster.u32 b, %1, %2;\n\t"
-      "st.shared::cluster.v2.f32 [s], {%3, %4};\n\t"
-      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [b];\n\t}" ::"r"(smem_addr(slot)),
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [s], {%3, %4}, [b];\n\t}" ::"r"(smem_addr(slot)),
       "r"(smem_addr(bar)), "r"(rank), "f"(v.x), "f"(v.y)
       : "memory");
 }
+// Arrives at this CTA's `bar` and has it wait for `bytes` besides.
+LZ_DEV void mbar_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}" ::"r"(smem_addr(bar)),
+               "r"(bytes)
+               : "memory");
+}
+
 // Waits for phase `parity` of `bar`, 4 s at most. A wait that gives up sets
 // `failed`, and the CTA's other waits then return at once: the kernel runs to its
 // end and leaves NaN.
 template <bool CLUSTER>
-LZ_DEV void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+LZ_DEV bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  return done != 0;
+}
+
+template <bool CLUSTER>
+__device__ __noinline__ void ring_wait_on(uint32_t bar, uint32_t parity, volatile int* failed) {
   unsigned long long began = 0;
-  for (uint32_t it = 0; it < 0xffffffffu; ++it) {
-    uint32_t done;
-    if (CLUSTER)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(done)
-          : "r"(smem_addr(bar)), "r"(parity)
-          : "memory");
-    else
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(done)
-          : "r"(smem_addr(bar)), "r"(parity)
-          : "memory");
-    if (done || *failed) return;
-    if (it % 64 == 63) {
+  for (uint32_t it = 1; it; ++it) {
+    if (try_wait<CLUSTER>(bar, parity) || *failed) return;
+    if (it % 64 == 0) {
       const unsigned long long now = globaltimer();
       if (!began) began = now;
       if (now - began > kWaitNs) break;
     }
   }
   *failed = 1;
+}
+
+template <bool CLUSTER>
+LZ_DEV void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  if (!try_wait<CLUSTER>(smem_addr(bar), parity)) ring_wait_on<CLUSTER>(smem_addr(bar), parity, failed);
+}
+
+// After a wait that gave up: copies still in flight land before the CTA ends.
+LZ_DEV void drain_copies() {
+  const unsigned long long began = globaltimer();
+  for (uint32_t it = 0; it < 100000000u && globaltimer() - began < 20000000ull; ++it) {
+  }
 }
 
 // Two fp32 operations an instruction.
@@ -820,6 +861,27 @@ LZ_DEV RowSum slow_sum(const T* x, long long n, float c) {
   return {m, 0.f, s};
 }
 
+// Two rows ahead the teacher's list goes to L2, and then the logits at its ids:
+// read only when they are needed, each took up to 3 us behind the rows' stream.
+LZ_DEV void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+LZ_DEV void touch_list(const LzLossArgs& a, long long r) {
+  const int id_bytes = a.ids64 ? 8 : 4, t_bytes = a.teacher_dtype == LZ_F32 ? 4 : 2;
+  for (int k = threadIdx.x % 32 * 16; k < a.top; k += 512) {  // one entry of each 128 bytes at least
+    prefetch_l2(static_cast<const char*>(a.ids) + (r * a.top + k) * id_bytes);
+    prefetch_l2(static_cast<const char*>(a.teacher) + (r * a.top + k) * t_bytes);
+  }
+}
+
+template <typename T>
+LZ_DEV void touch_logits(const LzLossArgs& a, const T* x, long long r) {
+#pragma unroll 4
+  for (int k = threadIdx.x % 32; k < a.top; k += 32) {
+    const long long id = load_id(a.ids, a.ids64, r * a.top + k);
+    if (id >= 0 && id < a.vocab) prefetch_l2(x + id);
+  }
+}
+
 // A row's scalars, fetched a row ahead.
 template <typename T, int KIND>
 LZ_DEV void prepare_params(const LzLossArgs& a, const StreamPlan& p, const T* x, long long r, RowParams& out, TopView t,
@@ -842,53 +904,79 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const StreamPlan& p, const T* x,
   }
   float m = -INFINITY;
   bool bad = false;
-  for (int k = lane; k < a.top; k += 32) {
-    const long long id = load_id(a.ids, a.ids64, r * a.top + k);
-    const float v = id < 0 ? -INFINITY : top_value(a, r, k);
-    const bool in = id >= 0 && id < a.vocab;
-    bad |= id >= a.vocab;
-    t.id[k] = in ? (int)id : -1;
-    t.z[k] = in ? Elem<T>::get(x[id]) : 0.f;
-    t.q[k] = v;
-    m = fmaxf(m, v);
+  for (int first = 0; first < a.top; first += 128) {  // four entries a lane at a time: their loads run together
+    long long id[4];
+    float v[4];
+    T z[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = first + 32 * u + lane;
+      id[u] = k < a.top ? load_id(a.ids, a.ids64, r * a.top + k) : -1;
+      v[u] = k < a.top ? top_value(a, r, k) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) z[u] = id[u] >= 0 && id[u] < a.vocab ? x[id[u]] : Elem<T>::put(0.f);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = first + 32 * u + lane;
+      if (k >= a.top) break;
+      if (id[u] < 0) v[u] = -INFINITY;
+      bad |= id[u] >= a.vocab;
+      t.id[k] = id[u] >= 0 && id[u] < a.vocab ? (int)id[u] : -1;
+      t.z[k] = Elem<T>::get(z[u]);
+      t.q[k] = v[u];
+      m = fmaxf(m, v[u]);
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   bad = __any_sync(~0u, bad);
+  // Sums over e = exp(v - m); q = e / s.
   float s = 0.f;
-  for (int k = lane; k < a.top; k += 32) s += m == -INFINITY ? 0.f : expf(t.q[k] - m);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  const float inv = s > 0.f || s != s ? 1.f / s : 0.f;
-  const double logsum = log((double)s);
-  double q_logq = 0.0, q_z = 0.0, q_sum = 0.0;
+  double e_v = 0.0, e_z = 0.0;
   for (int k = lane; k < a.top; k += 32) {
-    const float v = t.q[k], q = m == -INFINITY ? 0.f : expf(v - m) * inv;
-    t.q[k] = q;
-    t.share[k] = t.id[k] < 0 ? -1.f : q;
-    if (q != 0.f) {  // NaN counts
-      q_logq += (double)q * ((double)v - m - logsum);
-      q_z += (double)q * ((double)t.z[k] * (double)c);
-      q_sum += (double)q;
+    const float v = t.q[k] - m, e = m == -INFINITY ? 0.f : expf(v);
+    t.q[k] = e;
+    if (e != 0.f) {  // NaN counts
+      s += e;
+      e_v += (double)e * (double)v;
+      e_z += (double)e * ((double)t.z[k] * (double)c);
     }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    q_logq += __shfl_xor_sync(~0u, q_logq, o);
-    q_z += __shfl_xor_sync(~0u, q_z, o);
-    q_sum += __shfl_xor_sync(~0u, q_sum, o);
+    s += __shfl_xor_sync(~0u, s, o);
+    e_v += __shfl_xor_sync(~0u, e_v, o);
+    e_z += __shfl_xor_sync(~0u, e_z, o);
   }
-  // Does an id stand in the list twice? Then its first entry gets all shares.
-  for (int k = lane; k < p.hash; k += 32) hash[k] = -1;
-  __syncwarp();
-  bool twice = false;
+  const float inv = s > 0.f || s != s ? 1.f / s : 0.f;
   for (int k = lane; k < a.top; k += 32) {
-    const int id = t.id[k];
-    if (id < 0) continue;
-    for (unsigned h = (unsigned)id * 2654435761u >> 7;; ++h) {  // ends: the table is twice the list
-      const int was = atomicCAS(hash + (h & (p.hash - 1)), -1, id);
-      twice |= was == id;
-      if (was == -1 || was == id) break;
+    const float q = t.q[k] * inv;
+    t.q[k] = q;
+    t.share[k] = t.id[k] < 0 ? -1.f : q;
+  }
+  __syncwarp();
+  // Does an id stand in the list twice? Then its first entry gets all shares.
+  bool twice = false;
+  if (a.top <= kSmallList) {
+    for (int k = lane; k < a.top; k += 32) {
+      const int id = t.id[k];
+      int same = 0;
+#pragma unroll 8
+      for (int o = 0; o < a.top; ++o) same += t.id[o] == id;
+      twice |= id >= 0 && same > 1;
+    }
+  } else {
+    for (int k = lane; k < p.hash; k += 32) hash[k] = -1;
+    __syncwarp();
+    for (int k = lane; k < a.top; k += 32) {
+      const int id = t.id[k];
+      if (id < 0) continue;
+      for (unsigned h = (unsigned)id * 2654435761u >> 7;; ++h) {  // ends: the table is twice the list
+        const int was = atomicCAS(hash + (h & (p.hash - 1)), -1, id);
+        twice |= was == id;
+        if (was == -1 || was == id) break;
+      }
     }
   }
   if (__any_sync(~0u, twice)) {
@@ -904,6 +992,10 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const StreamPlan& p, const T* x,
       t.share[k] = first ? q : -1.f;
     }
   }
+  float whole, part;
+  log2_parts(s, &whole, &part);
+  const double q_sum = (double)s * (double)inv;
+  const double q_logq = s == 0.f ? 0.0 : e_v * (double)inv - q_sum * ((double)whole + (double)part) * kLn2, q_z = e_z * (double)inv;
   if (lane == 0) {
     out.weight = (a.weights ? (double)a.weights[r] : 1.0) * a.work[0];
     out.slope = bad ? NAN : m == -INFINITY ? 0.f : (float)-out.weight;
@@ -912,7 +1004,7 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const StreamPlan& p, const T* x,
   __syncwarp();
 }
 
-constexpr int kBatch = 4;  // vectors a thread has in work at a time
+constexpr int kBatch = 3;  // vectors a thread has in work at a time
 
 // Sum over a thread's elements of 2^(x c - ref). ref is not the running maximum:
 // it is taken from the first batch and moves only when a batch's maximum is more
@@ -933,12 +1025,6 @@ struct LazySum {
   }
 };
 
-template <typename T>
-LZ_DEV uint4 minus_infinity() {
-  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : Elem<T>::N == 8 && std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-  return make_uint4(w, w, w, w);
-}
-
 template <typename T, int U>
 LZ_DEV void batch_sum(const uint4* w, uint64_t c2, uint64_t neg_ref, uint64_t* out) {
 #pragma unroll
@@ -954,12 +1040,14 @@ LZ_DEV void batch_sum(const uint4* w, uint64_t c2, uint64_t neg_ref, uint64_t* o
   }
 }
 
+// `first` (of a row): nothing to go by, so the maximum comes first.
 template <typename T, int U>
-LZ_DEV void take_batch(LazySum& s, const uint4* w, float c) {
+LZ_DEV void take_batch(LazySum& s, const uint4* w, float c, bool first) {
   const uint64_t c2 = pair(c, c);
   float m = vector_max<T>(w[0]);
 #pragma unroll
   for (int u = 1; u < U; ++u) m = fmaxf(m, vector_max<T>(w[u]));
+  if (first && m > s.limit) s.raise(m, c);
   uint64_t part[2] = {0, 0};
   batch_sum<T, U>(w, c2, s.neg_ref, part);
   if (m > s.limit) {
@@ -970,11 +1058,17 @@ LZ_DEV void take_batch(LazySum& s, const uint4* w, float c) {
   s.sum[0] = add2(s.sum[0], part[0]), s.sum[1] = add2(s.sum[1], part[1]);
 }
 
+// Warps beside the W that take chunks: one feeds the ring, one has the rows'
+// scalars; DISTILL's lists take one more (about 9000 cycles for 64 entries, of
+// the 15000 that a slice of 150 KB takes; on one warp they were the bound).
+template <int KIND>
+constexpr int kHelpers = KIND == LZ_LOSS_DISTILL ? 3 : 2;
+
 template <typename T, int KIND, bool GRAD, int W>
-__global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_constant__ LzLossArgs a,
+__global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(const __grid_constant__ LzLossArgs a,
                                                                  const __grid_constant__ StreamPlan plan) {
   constexpr int N = Elem<T>::N, kTake = W * 32;
-  constexpr int kChunkVecs = kBatch / 2 * kTake, kChunk = 16 * kChunkVecs;
+  constexpr int kChunkVecs = kBatch * kTake, kChunk = 16 * kChunkVecs;
   extern __shared__ __align__(128) char smem[];
   StreamShared& sh = *reinterpret_cast<StreamShared*>(smem);
   char* const lists = smem + sizeof(StreamShared);
@@ -999,6 +1093,10 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
     else h.row = -1;
     return h;
   };
+  auto view = [&](int k) {
+    float* f = reinterpret_cast<float*>(lists) + k * 4 * a.top;
+    return TopView{reinterpret_cast<int*>(f), f + a.top, f + 2 * a.top, f + 3 * a.top};
+  };
   if (tid == 0) {
     for (int s = 0; s < plan.slots; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -1006,13 +1104,15 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
     }
     for (int k = 0; k < 2; ++k) {
       mbar_init(&sh.parts[k], W);
-      mbar_init(&sh.peers[k], ranks);
+      mbar_init(&sh.peers[k], 1);
       mbar_init(&sh.dense[k], 1);
+      mbar_init(&sh.ready[k], 1);
+      mbar_init(&sh.used[k], 1);
     }
     fence_mbar_init();
     *failed = 0;
   }
-  if (tid >= (W + 1) * 32 && lane < 2) sh.heads[lane] = head_at(cluster + lane * clusters);
+  if (warp == W + 1 && lane < 2) sh.heads[lane] = head_at(cluster + lane * clusters);
   cluster_sync();
 
   if (warp == W) {  // ---- streams the slices into the ring
@@ -1031,10 +1131,7 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
         }
         h = next;
       }
-      if (*failed) {  // what is in flight lands before the CTA ends
-        for (uint32_t s = 0; s < (uint32_t)plan.slots; ++s)
-          if (round || s < slot) mbar_wait(&sh.full[s], (s < slot ? round : round - 1) & 1, 1u << 20);
-      }
+      if (*failed) drain_copies();
     }
     __syncwarp();
   } else if (warp < W) {  // ---- sums, then the dense gradient
@@ -1045,27 +1142,24 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
     int done = 0;  // chunks of the row that are in `sum`
     // Chunks [done, upto) of a row, two at a time.
     auto take = [&](const RowHead& h, int upto) {
-      for (; done < upto; done += 2) {
-        uint4 w[kBatch];
+      for (; done < upto; ++done) {
+        const int vecs = h.count - done * kChunkVecs;
+        ring_wait<false>(&sh.full[slot], round & 1, failed);
+        const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk) + tid;
+        if (vecs >= kChunkVecs) {
+          uint4 w[kBatch];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          w[2 * b] = w[2 * b + 1] = minus_infinity<T>();
-          if (done + b < upto) {
-            ring_wait<false>(&sh.full[slot], round & 1, failed);
-            const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk);
-            const int vecs = h.count - (done + b) * kChunkVecs;
-            if (tid < vecs) w[2 * b] = v[tid];
-            if (tid + kTake < vecs) w[2 * b + 1] = v[tid + kTake];
-            if (!GRAD) {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh.empty[slot]);
-            }
-            if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
-          }
+          for (int u = 0; u < kBatch; ++u) w[u] = v[u * kTake];
+          take_batch<T, kBatch>(sum, w, c, done == 0);
+        } else {
+          for (int j = tid; j < vecs; j += kTake, v += kTake) take_batch<T, 1>(sum, v, c, true);
         }
-        take_batch<T, kBatch>(sum, w, c);
+        if (!GRAD) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[slot]);
+        }
+        if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
       }
-      done = min(done, upto);
     };
     uint32_t turn = 0;
     for (;; ++turn) {
@@ -1110,12 +1204,13 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
           for (int j = tid; j < kChunkVecs; j += kTake)
             if (j < vecs) st_cs_v4(o + j, make_uint4(0, 0, 0, 0));
         } else if (d.base == 0.f) {
-          uint4 w[kBatch / 2];
+          uint4 w[kBatch];
 #pragma unroll
-          for (int u = 0; u < kBatch / 2; ++u)
+          for (int u = 0; u < kBatch; ++u)
             if (tid + u * kTake < vecs) w[u] = v[tid + u * kTake];
 #pragma unroll
-          for (int u = 0; u < kBatch / 2; ++u) {
+          for (int u = 0; u < kBatch; ++u) {
+            if (u * kTake >= vecs) break;
             uint64_t p[N / 2];
             float e[N];
             unpack_pairs<T>(w[u], p);
@@ -1157,12 +1252,20 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
         if (single >= 0) out[single] = Elem<T>::put(0.f);
       }
     }
-  } else {  // ---- joins the sums; the rows' scalars, outputs and sparse entries
-    auto view = [&](int k) {
-      float* f = reinterpret_cast<float*>(lists) + k * 4 * a.top;
-      return TopView{reinterpret_cast<int*>(f), f + a.top, f + 2 * a.top, f + 3 * a.top};
-    };
+  } else if (KIND == LZ_LOSS_DISTILL && warp == W + 2) {  // ---- the teacher's lists, a row ahead
     int* const hash = reinterpret_cast<int*>(lists) + 8 * a.top;
+    long long r, to_come;
+    for (uint32_t turn = 0; row_at(cluster + (long long)turn * clusters, &r); ++turn) {
+      const int k = turn & 1;
+      if (row_at(cluster + (long long)(turn + 2) * clusters, &to_come)) touch_list(a, to_come);
+      if (turn >= 2) ring_wait<false>(&sh.used[k], ((turn - 2) >> 1) & 1, failed);
+      prepare_params<T, KIND>(a, plan, row_of<T>(a, r), r, sh.params[k], view(k), hash, c);
+      if (lane == 0) mbar_arrive(&sh.ready[k]);
+      if (row_at(cluster + (long long)(turn + 1) * clusters, &to_come))
+        touch_logits(a, row_of<T>(a, to_come), to_come);
+    }
+    __syncwarp();
+  } else {  // ---- joins the sums; the rows' scalars, outputs and sparse entries
     double loss = 0.0;
     RowHead before = {-1};  // the row whose dense part is being written, its slope, token and sum
     float before_slope = 0.f, before_xy = 0.f;
@@ -1188,7 +1291,8 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
       }
     };
     auto prepare = [&](const RowHead& h, int k) {
-      if (h.row >= 0) prepare_params<T, KIND>(a, plan, row_of<T>(a, h.row), h.row, sh.params, view(k), hash, c);
+      if (KIND != LZ_LOSS_DISTILL && h.row >= 0)
+        prepare_params<T, KIND>(a, plan, row_of<T>(a, h.row), h.row, sh.params[k], TopView{}, nullptr, c);
     };
     prepare(sh.heads[0], 0);
     uint32_t turn = 0;
@@ -1201,6 +1305,7 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
       float2 v = sh.warp_part[k][lane % W];
       lanes_join(v.x, v.y, W);
       if (ranks > 1) {
+        if (lane == 0) mbar_expect(&sh.peers[k], ranks * (uint32_t)sizeof(float2));
         if (lane < ranks) send_to_peer(&sh.peer_part[k][rank], v, &sh.peers[k], lane);
         __syncwarp();
         ring_wait<true>(&sh.peers[k], (turn >> 1) & 1, failed);
@@ -1209,7 +1314,8 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
       }
       RowSum n = {0.f, v.x, v.y};
       if (isinf(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
-      const RowParams& p = sh.params;
+      if (KIND == LZ_LOSS_DISTILL) ring_wait<false>(&sh.ready[k], (turn >> 1) & 1, failed);
+      const RowParams& p = sh.params[k];
       const Norm norm = n.norm();
       const double logp2 = p.token < 0 ? (double)NAN : ((double)p.xy - (double)norm.base) * (double)c - norm.lse2;
       PolicyOut o = {0.f, 0.f, false};
@@ -1221,6 +1327,8 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
         mbar_arrive(&sh.dense[k]);
       }
       sparse(k ^ 1);
+      __syncwarp();
+      if (KIND == LZ_LOSS_DISTILL && turn && lane == 0) mbar_arrive(&sh.used[k ^ 1]);  // by the row before
       double kl = 0.0;
       if (KIND == LZ_LOSS_DISTILL) {
         kl = p.q_logq - kLn2 * (p.q_z - p.q_sum * norm.lse2);
@@ -1300,6 +1408,159 @@ __global__ void __launch_bounds__((W + 2) * 32, 1) stream_kernel(const __grid_co
     __syncwarp();
   }
   cluster_sync();  // no CTA leaves while a peer may still write to it
+}
+
+// The gradient alone, for rows whose sums and slopes are known (LOGP, POLICY). A
+// chunk is a piece of work of its own: what it takes from its row travels in the
+// ring slot's head. The feeding warp works the heads of its next 32 chunks out
+// at once, a lane each, and issues them in turn.
+struct ChunkHead {
+  void* out;             // first vector of the chunk
+  const void* row;       // logits of the row and, with `singles`, its gradient row
+  void* out_row;
+  int vecs, token_vec, token_at;  // the vector that holds the token (-1: none) and its place in it
+  int singles, lead, tail;        // 1: the row's single elements go with this chunk
+  float f, base, ref, token_value;
+  int token;
+};
+
+struct alignas(128) GradShared {
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  ChunkHead heads[kMaxSlots];
+  int failed;
+};
+
+template <typename T, int KIND, int W>
+__global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __grid_constant__ LzLossArgs a, int slots) {
+  constexpr int N = Elem<T>::N, kTake = W * 32;
+  constexpr int kChunkVecs = kBatch * kTake, kChunk = 16 * kChunkVecs;
+  extern __shared__ __align__(128) char smem[];
+  GradShared& sh = *reinterpret_cast<GradShared*>(smem);
+  char* const ring = smem + sizeof(GradShared);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const float c = (float)(kLog2e * (double)a.inv_temperature);
+  volatile int* const failed = &sh.failed;
+  const float up = a.upstream ? *a.upstream : 1.f;
+  if (!a.fresh && up == 1.f) return;
+  if (tid == 0) {
+    for (int s = 0; s < slots; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], W);
+    }
+    fence_mbar_init();
+    *failed = 0;
+  }
+  __syncthreads();
+  const int per_row = (int)((a.vocab / N + kChunkVecs - 1) / kChunkVecs);  // chunks of a row, the last of them maybe empty
+  const long long all = a.rows * per_row;
+
+  if (warp == W) {
+    uint32_t slot = 0, round = 0;
+    for (long long first = blockIdx.x; first < all; first += 32ll * gridDim.x) {
+      const long long g = first + (long long)lane * gridDim.x;
+      ChunkHead h = {};
+      const char* from = nullptr;
+      if (g < all) {
+        const long long r = g / per_row;
+        const int piece = (int)(g % per_row);
+        const T* x = row_of<T>(a, r);
+        T* out = static_cast<T*>(a.grad) + r * a.vocab;
+        const double2 norm = work_norm(a)[r];
+        const long long y = load_id(a.ids, a.ids64, r);
+        const double slope = row_slope_for<KIND>(a, r, y, up);
+        const Split<T> sp(x, a.vocab);
+        h.vecs = max(0, min(kChunkVecs, sp.vecs - piece * kChunkVecs));
+        const long long at = sp.lead + (long long)piece * kChunkVecs * N;
+        h.out = out + at;
+        h.row = x, h.out_row = out;
+        h.singles = piece == 0, h.lead = sp.lead, h.tail = (int)(a.vocab - sp.lead) % N;
+        h.base = (float)norm.x, h.ref = (float)norm.y;
+        const double left = (double)h.ref - norm.y;  // at most half a step of ref: 2^left is 1 + left ln 2
+        h.f = slope == 0.0 ? 0.f : (float)(-slope * a.inv_temperature * (1.0 + left * kLn2));
+        h.token = -1, h.token_vec = -1;
+        if (y >= 0 && y < a.vocab && h.f != 0.f) {
+          const long long in = y - at;
+          if (in >= 0 && in < (long long)h.vecs * N) h.token_vec = (int)(in / N), h.token_at = (int)(in % N);
+          else if (h.singles && (y < sp.lead || y >= a.vocab - h.tail)) h.token = (int)y;
+          if (h.token_vec >= 0 || h.token >= 0) {
+            const float p = exp2_fast(fmaf(Elem<T>::get(x[y]) - h.base, c, -h.ref)) * (float)(1.0 + left * kLn2);
+            h.token_value = (float)(slope * a.inv_temperature) * (1.f - p);
+          }
+        }
+        from = reinterpret_cast<const char*>(x + at);
+      }
+      for (int l = 0; l < 32 && first + (long long)l * gridDim.x < all; ++l) {
+        if (lane == l) {
+          if (round) ring_wait<false>(&sh.empty[slot], (round - 1) & 1, failed);
+          if (!*failed) {
+            sh.heads[slot] = h;
+            if (h.f != 0.f && h.vecs > 0) bulk_g2s(ring + (size_t)slot * kChunk, from, h.vecs * 16, &sh.full[slot]);
+            else mbar_arrive(&sh.full[slot]);  // nothing to read
+          }
+        }
+        __syncwarp();
+        if (++slot == (uint32_t)slots) slot = 0, ++round;
+      }
+    }
+    if (*failed) drain_copies();
+    __syncwarp();
+  } else {
+    uint32_t slot = 0, round = 0;
+    for (long long g = blockIdx.x; g < all; g += gridDim.x) {
+      ring_wait<false>(&sh.full[slot], round & 1, failed);
+      const ChunkHead& h = sh.heads[slot];
+      const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk) + tid;
+      uint4* o = static_cast<uint4*>(h.out) + tid;
+      const int vecs = *failed ? 0 : h.vecs;
+      const float f = *failed ? 0.f : h.f, base = h.base, ref = h.ref;
+      const int token_vec = h.token_vec;
+      if (f == 0.f) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (tid + u * kTake < vecs) st_cs_v4(o + u * kTake, make_uint4(0, 0, 0, 0));
+      } else {
+        uint4 w[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (tid + u * kTake < vecs) w[u] = v[u * kTake];
+        const uint64_t c2 = pair(c, c), f2 = pair(f, f), off2 = pair(-ref, -ref);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (u * kTake >= vecs) break;
+          float e[N];
+          if (base == 0.f) {
+            uint64_t p[N / 2];
+            unpack_pairs<T>(w[u], p);
+#pragma unroll
+            for (int q = 0; q < N / 2; ++q) {
+              float lo, hi;
+              unpair(fma2(p[q], c2, off2), lo, hi);
+              unpair(mul2(f2, pair(exp2_fast(lo), exp2_fast(hi))), e[2 * q], e[2 * q + 1]);
+            }
+          } else {
+            Elem<T>::unpack(w[u], e);
+#pragma unroll
+            for (int q = 0; q < N; ++q) e[q] = f * exp2_fast(fmaf(e[q] - base, c, -ref));
+          }
+          if (tid + u * kTake < vecs) st_cs_v4(o + u * kTake, Elem<T>::pack(e));
+        }
+        if (token_vec >= 0 && token_vec % kTake == tid)  // over its vector, by the thread that wrote it
+          reinterpret_cast<T*>(static_cast<uint4*>(h.out) + token_vec)[h.token_at] = Elem<T>::put(h.token_value);
+      }
+      if (h.singles && tid < h.lead + h.tail && !*failed) {
+        const long long i = tid < h.lead ? tid : a.vocab - h.tail + tid - h.lead;
+        float e = 0.f;
+        if (f != 0.f) e = i == h.token ? h.token_value : f * exp2_fast(fmaf(Elem<T>::get(static_cast<const T*>(h.row)[i]) - base, c, -ref));
+        static_cast<T*>(h.out_row)[i] = Elem<T>::put(e);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[slot]);
+      if (++slot == (uint32_t)slots) slot = 0, ++round;
+    }
+    if (*failed)  // a wait gave up: the gradient is NaN, not stale
+      for (long long i = tid; i < a.rows * a.vocab; i += kTake)
+        static_cast<T*>(a.grad)[i] = Elem<T>::put(NAN);
+  }
 }
 
 // Preference loss of one pair a CTA: sums of its two sequences' log-probabilities
@@ -1382,8 +1643,20 @@ struct StreamLaunch {
   size_t smem;
 };
 
+// Whether rows can be streamed: not small, and each row and its gradient at the
+// same offset from a 16-byte border.
+template <typename T>
+bool streams(const LzLossArgs* a, bool grad) {
+  const long long size = sizeof(T), row = a->vocab * size;
+  if (row < 16384 || a->rows > INT32_MAX) return false;
+  if (!grad) return true;
+  return ((uintptr_t)a->logits ^ (uintptr_t)a->grad) % 16 == 0 &&
+         (a->inner >= a->rows || (a->outer_stride * size - a->inner * row) % 16 == 0) &&
+         (a->inner <= 1 || (a->inner_stride * size - row) % 16 == 0);
+}
+
 constexpr int kStreamWarps = 16;
-constexpr int kChunk = 16 * kBatch / 2 * kStreamWarps * 32;  // bytes of a ring slot: half a batch of every thread
+constexpr int kChunk = 16 * kBatch * kStreamWarps * 32;  // bytes of a ring slot: a batch of every thread
 constexpr int kSharedMax = 232448;
 constexpr int kMaxDevices = 64;
 
@@ -1391,13 +1664,9 @@ template <typename T, int KIND, bool GRAD>
 int plan_stream(const LzLossArgs* a, StreamLaunch* l, bool* fits) {
   *fits = false;
   const long long row = a->vocab * (long long)sizeof(T);
-  if (row < 16384 || a->rows > INT32_MAX) return LZE_OK;
-  if (GRAD && ((((uintptr_t)a->logits ^ (uintptr_t)a->grad) % 16) ||
-               (a->inner < a->rows && (a->outer_stride * (long long)sizeof(T) - a->inner * row) % 16) ||
-               (a->inner > 1 && (a->inner_stride * (long long)sizeof(T) - row) % 16)))
-    return LZE_OK;
+  if (!streams<T>(a, GRAD)) return LZE_OK;
   int hash = 0;
-  if (KIND == LZ_LOSS_DISTILL)
+  if (KIND == LZ_LOSS_DISTILL && a->top > kSmallList)
     for (hash = 32; hash < 2 * a->top;) hash *= 2;
   const int fixed = (int)sizeof(StreamShared) + list_bytes(KIND, a->top, hash);
   const int slots = (kSharedMax - fixed) / kChunk < kMaxSlots ? (kSharedMax - fixed) / kChunk : kMaxSlots;
@@ -1412,7 +1681,7 @@ int plan_stream(const LzLossArgs* a, StreamLaunch* l, bool* fits) {
       cudaLaunchAttribute at[1] = {};
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim = {1u << k, 1, 1};
-      cfg.gridDim = dim3(148 * 8), cfg.blockDim = dim3((kStreamWarps + 2) * 32), cfg.dynamicSmemBytes = kSharedMax;
+      cfg.gridDim = dim3(148 * 8), cfg.blockDim = dim3((kStreamWarps + kHelpers<KIND>) * 32), cfg.dynamicSmemBytes = kSharedMax;
       cfg.attrs = at, cfg.numAttrs = 1;
       int g = 0;
       LZ_CUDA_TRY(cudaOccupancyMaxActiveClusters(&g, kernel, &cfg));
@@ -1434,7 +1703,7 @@ int plan_stream(const LzLossArgs* a, StreamLaunch* l, bool* fits) {
     chunks = (int)((slice + 16 + kChunk - 1) / kChunk);
   }
   if (best == 0.0) return LZE_OK;
-  l->plan = {slots, (slots - chunks) / 2 * 2, a->rows > l->clusters, hash};
+  l->plan = {slots, slots - chunks, a->rows > l->clusters, hash};
   l->smem = fixed + (size_t)slots * kChunk;
   *fits = true;
   return LZE_OK;
@@ -1446,7 +1715,7 @@ int launch_stream(const LzLossArgs* a, const StreamLaunch& l, cudaStream_t s) {
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim = {(unsigned)l.ranks, 1, 1};
-  cfg.gridDim = dim3(l.clusters * l.ranks), cfg.blockDim = dim3((kStreamWarps + 2) * 32);
+  cfg.gridDim = dim3(l.clusters * l.ranks), cfg.blockDim = dim3((kStreamWarps + kHelpers<KIND>) * 32);
   cfg.dynamicSmemBytes = l.smem, cfg.stream = s, cfg.attrs = at, cfg.numAttrs = 1;
   LZ_CUDA_TRY(cudaLaunchKernelEx(&cfg, stream_kernel<T, KIND, GRAD, kStreamWarps>, *a, l.plan));
   return LZE_OK;
@@ -1478,8 +1747,29 @@ int launch_forward(const LzLossArgs* a, cudaStream_t s) {
 }
 
 template <typename T, int KIND>
+int launch_stream_grad(const LzLossArgs* a, cudaStream_t s) {
+  auto kernel = stream_grad_kernel<T, KIND, kStreamWarps>;
+  static std::atomic<int> sms[kMaxDevices];
+  int n = sms[a->device].load(std::memory_order_acquire);
+  if (!n) {
+    LZ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMax));
+    LZ_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, a->device));
+    sms[a->device].store(n, std::memory_order_release);
+  }
+  // Four chunks ahead: with nine, as many as fit, the reads queue in front of the
+  // writes (4096 rows of 151936 in bf16, half of them read: 408 us a step against 432).
+  constexpr int slots = 4;
+  static_assert(slots * kChunk + sizeof(GradShared) <= kSharedMax && slots <= kMaxSlots, "ring");
+  kernel<<<n, (kStreamWarps + 1) * 32, sizeof(GradShared) + (size_t)slots * kChunk, s>>>(*a, slots);
+  LZ_CUDA_TRY(cudaGetLastError());
+  return LZE_OK;
+}
+
+template <typename T, int KIND>
 int launch_backward(const LzLossArgs* a, cudaStream_t s) {
   if (!a->rows) return LZE_OK;
+  if constexpr (KIND != LZ_LOSS_DISTILL)
+    if (streams<T>(a, true) && a->device < kMaxDevices) return launch_stream_grad<T, KIND>(a, s);
   int grid = 0;
   if (const int rc = grid_for(a->device, a->rows, &grid)) return rc;
   backward_kernel<T, KIND><<<grid, kThreads, top_bytes(a), s>>>(*a);
