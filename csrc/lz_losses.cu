@@ -92,13 +92,15 @@ struct Elem<__half> {
 };
 
 // Running maximum and sum of a softmax: sum_j 2^(x_j c - ref), where ref is the
-// maximum (0 while it is -inf, so that rows of -inf sum to 0 and not to NaN).
-// A NaN or +inf among the logits makes the sum NaN.
+// maximum, rounded to an integer so that sums are brought to another reference
+// without a rounding (0 while it is -inf, so that rows of -inf sum to 0 and not
+// to NaN). A NaN or +inf among the logits makes the sum NaN.
 struct Running {
   float max, ref, sum;
   LZ_DEV void init() { max = -INFINITY, ref = 0.f, sum = 0.f; }
   LZ_DEV void raise(float m) {
-    if (m > max) {
+    if (m > max + 0.5f) {
+      m = rintf(m);
       sum *= exp2_fast(max - m);
       max = m, ref = m;
     }
@@ -392,7 +394,7 @@ LZ_DEV double token_scalars(const LzLossArgs& a, const T* x, long long r, long l
   const bool there = y < a.vocab;  // otherwise every output of the row is NaN
   const double logp = there ? row_log2p(x, y, n, c) * kLn2 : (double)NAN;
   a.logp[r] = (float)logp;
-  if (KIND == LZ_LOSS_LOGP) return 0.0;
+  if (KIND == LZ_LOSS_LOGP) return logp;
   const double w = (a.weights ? (double)a.weights[r] : 1.0) * a.work[0];
   const double adv = a.advantages[r], ratio = exp(logp - (double)a.old_logp[r]);
   const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
@@ -1007,7 +1009,7 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const StreamPlan& p, const T* x,
 constexpr int kBatch = 3;  // vectors a thread has in work at a time
 
 // Sum over a thread's elements of 2^(x c - ref). ref is not the running maximum:
-// it is taken from the first batch and moves only when a batch's maximum is more
+// it is taken from the first batch (as an integer, as above) and moves only when a batch's maximum is more
 // than 2^16 above it, which fp32 has room for (2^16 times the vocabulary), so the
 // exponentials of a batch wait for no maximum and the branch is seldom taken.
 struct LazySum {
@@ -1018,9 +1020,9 @@ struct LazySum {
     limit = -3e38f / fmaxf(c, 1.f);  // below this x c is beyond 32 bits: such entries count nothing
   }
   LZ_DEV void raise(float m, float c) {
-    const float f = exp2_fast(ref - m * c);
+    const float to = rintf(m * c), f = exp2_fast(ref - to);
     sum[0] = mul2(sum[0], pair(f, f)), sum[1] = mul2(sum[1], pair(f, f));
-    ref = m * c, neg_ref = pair(-ref, -ref);
+    ref = to, neg_ref = pair(-ref, -ref);
     limit = m + 16.f / c;
   }
 };
@@ -1360,7 +1362,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         if (KIND == LZ_LOSS_DISTILL) a.kl[h.row] = (float)kl;
         if (KIND != LZ_LOSS_LOGP) loss += p.weight * each;
         work_norm(a)[h.row] = make_double2(norm.base, norm.lse2);
-        work_slope(a)[h.row] = (double)slope;
+        work_slope(a)[h.row] = KIND == LZ_LOSS_LOGP ? logp2 * kLn2 : (double)slope;
       }
       before = h, before_n = n, before_slope = slope, before_xy = p.xy, before_token = p.token;
       __syncwarp();
@@ -1573,6 +1575,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   const long long n = a.rows;
   const long long pair = blockIdx.x;
   float* slope = reinterpret_cast<float*>(a.work + 1 + a.pairs);
+  const double* logp = a.logp_work + LZ_LOSS_WORK_HEAD + 2 * n;  // as work_slope
   auto offset = [&](long long s) { return a.offsets ? load_id(a.offsets, a.offsets64, s) : s * a.length; };
   long long begin[2], end[2];
   double reward[2], per[2];
@@ -1584,7 +1587,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
     if (begin[k] < 0 || begin[k] > end[k] || end[k] > n) bad = true, begin[k] = end[k] = 0;
     double sum = 0.0, count = 0.0;
     for (long long r = begin[k] + threadIdx.x; r < end[k]; r += kThreads)
-      if (load_id(a.ids, a.ids64, r) >= 0) sum += (double)a.logp[r], count += 1.0;
+      if (load_id(a.ids, a.ids64, r) >= 0) sum += logp[r], count += 1.0;
     sum = block_sum(sum, red);
     count = block_sum(count, red);
     per[k] = a.normalized ? 1.0 / (count > 1.0 ? count : 1.0) : 1.0;

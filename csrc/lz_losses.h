@@ -40,7 +40,8 @@ struct LzLossArgs {
   float* kl;             // [rows] (POLICY with ref_logp, DISTILL)
   unsigned char* clipped;  // [rows] (POLICY)
   // [HEAD + ROW rows], 16-byte aligned: head, then per row its normaliser (two
-  // doubles), the slope of the loss in its log-probability, its loss, and its
+  // doubles), the slope of the loss in its log-probability (LOGP: that itself, in
+  // 64 bits, since sums of many are taken of it), its loss, and its
   // place in the order in which rows are taken (int)
   double* work;
   double denom;          // denominator; < 0: the sum of the weights
@@ -54,11 +55,12 @@ int lz_loss_forward(const struct LzLossArgs* a, cudaStream_t stream);
 // The gradient for another upstream value, from the statistics in `work`.
 int lz_loss_backward(const struct LzLossArgs* a, cudaStream_t stream);
 
-// Preference loss from the rows' log-probabilities (logp, ids as in LOGP):
+// Preference loss from the rows' log-probabilities (the `work` that lz_loss_forward
+// of LOGP left, ids as there):
 // sequences are [offsets[i], offsets[i+1]) or `length` rows each; the first
 // `pairs` are the chosen ones. Writes loss, rewards [2 pairs] and, in work, the slopes.
 struct LzPairArgs {
-  const float* logp;
+  const double* logp_work;
   const void* ids;
   const void* offsets;   // [2 pairs + 1] or null
   const float* ref_logp; // [2 pairs] or null

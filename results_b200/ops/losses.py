@@ -59,8 +59,8 @@ class _LossArgs(C.Structure):  # struct LzLossArgs
 
 
 class _PairArgs(C.Structure):  # struct LzPairArgs
-    _fields_ = [("logp", _p), ("ids", _p), ("offsets", _p), ("ref_logp", _p), ("loss", _p), ("rewards", _p),
-                ("work", _p), ("rows", _l), ("pairs", _l), ("length", _l), ("beta", _d), ("smoothing", _d),
+    _fields_ = [("logp_work", _p), ("ids", _p), ("offsets", _p), ("ref_logp", _p), ("loss", _p),
+                ("rewards", _p), ("work", _p), ("rows", _l), ("pairs", _l), ("length", _l), ("beta", _d), ("smoothing", _d),
                 ("normalized", _i), ("ids64", _i), ("offsets64", _i), ("device", _i)]
 
 
@@ -117,6 +117,8 @@ def _check_rows(what: str, name: str, t: torch.Tensor | None, shape, device, any
     """A value per row (or sequence) as contiguous fp32."""
     if t is None:
         return None
+    if t.dtype is torch.float32 and t.shape == shape and t.device == device and not t.requires_grad:
+        return t.contiguous()
     if not (t.is_floating_point() or any_type) or t.is_complex():
         raise TypeError(f"{what}: {name} is {t.dtype}; expected a floating-point type")
     if t.shape != shape:
@@ -125,7 +127,7 @@ def _check_rows(what: str, name: str, t: torch.Tensor | None, shape, device, any
         raise ValueError(f"{what}: {name} is on {t.device}, the logits on {device}")
     if t.requires_grad:
         raise ValueError(f"{what}: {name} requires a gradient, and this loss gives none to it; detach it")
-    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+    return t.to(torch.float32).contiguous()
 
 
 def _check_number(what: str, name: str, v, low: float, high: float = math.inf, open_low: bool = False) -> float:
@@ -157,8 +159,9 @@ def _check_denom(what: str, denom, device):
 
 # ---- native calls ---------------------------------------------------------------------------------------
 #
-# Small calls are bound by what runs on the host, so the arguments are built in one
-# go, once per call, and the backward pass takes the forward pass's.
+# Small calls are bound by what runs on the host: the arguments are built in one
+# go, the backward pass takes the forward pass's, and only the differentiable
+# output goes through autograd.
 
 
 def _ptr(t: torch.Tensor | None):
@@ -193,168 +196,114 @@ def _launch(fn: str, a, what: str) -> None:
         _native.check(rc, what)
 
 
-def _start(kind: int, logits: torch.Tensor, ids: torch.Tensor, temperature: float, denom=None, grad=None, teacher=None,
-           rows=(None, None, None, None), out=(None, None, None, None), numbers=(0.0, 0.0, 0.0)):
-    """Runs the forward pass; returns its arguments, the logits as they were read and the workspace."""
-    x, outer_stride, inner_stride, inner, n = _rows_of(logits)
-    work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=x.device)
-    old, adv, ref, weights = rows
-    loss, logp, kl, clipped = out
-    on_device = isinstance(denom, torch.Tensor)
-    a = _LossArgs(
-        x.data_ptr(), outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(grad), ids.data_ptr(), _ptr(teacher),
-        _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights), denom.data_ptr() if on_device else None, None, None, _ptr(loss),
-        _ptr(logp), _ptr(kl), _ptr(clipped), work.data_ptr(), -1.0 if denom is None or on_device else denom,
-        1.0 / temperature, *numbers, kind, _DTYPES[x.dtype], ids.dtype is torch.int64,
-        ids.shape[-1] if teacher is not None else 0, _DTYPES[teacher.dtype] if teacher is not None else 0,
-        x.device.index, 0)
-    _launch("lz_loss_forward", a, _NAMES[kind])
-    return a, x, work
-
-
-def _finish(a: _LossArgs, x: torch.Tensor, ids: torch.Tensor, work: torch.Tensor, shape, grad=None, upstream=None,
-            row_upstream=None, teacher=None) -> torch.Tensor:
-    """Runs the backward pass with the forward pass's arguments `a`; `grad` is what that left, if it did."""
-    if x.data_ptr() != a.logits:  # a saved tensor that came back from elsewhere
-        x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(x)
-    a.logits, a.ids, a.work, a.fresh = x.data_ptr(), ids.data_ptr(), work.data_ptr(), grad is None
-    if teacher is not None:
-        a.teacher = teacher.data_ptr()
-    if grad is None:
-        grad = torch.empty(shape, dtype=x.dtype, device=x.device)
-    a.grad, a.upstream, a.row_upstream = grad.data_ptr(), _ptr(upstream), _ptr(row_upstream)
-    _launch("lz_loss_backward", a, _NAMES[a.kind])
-    return grad
-
-
-def _grad_like(logits: torch.Tensor) -> torch.Tensor:
+def _empty_grad(logits: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(logits, memory_format=torch.contiguous_format)
 
 
-def _fp32(g: torch.Tensor) -> torch.Tensor:
-    return g if g.dtype is torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
+class _Call:
+    """One call: its arguments, its output `out`, and the tensors that the
+    backward pass reads (`keep`, until autograd has them)."""
+
+    def __init__(self, kind, logits, ids, temperature, out, logp=None, kl=None, clipped=None,
+                 rows=(None, None, None, None), teacher=None, denom=None, numbers=(0.0, 0.0, 0.0), fused=False):
+        x, outer_stride, inner_stride, inner, n = _rows_of(logits)
+        work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=x.device)
+        # the gradient for upstream 1, written by the forward pass
+        self.grad = _empty_grad(logits) if fused else None
+        self.out, self.shape = out, logits.shape
+        self.keep = (x, ids, work) if teacher is None else (x, ids, work, teacher)
+        old, adv, ref, weights = rows
+        on_device = isinstance(denom, torch.Tensor)
+        self.args = _LossArgs(
+            x.data_ptr(), outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(self.grad), ids.data_ptr(), _ptr(teacher),
+            _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights), denom.data_ptr() if on_device else None, None, None,
+            None if kind == LOGP else out.data_ptr(), _ptr(logp), _ptr(kl), _ptr(clipped), work.data_ptr(),
+            -1.0 if denom is None or on_device else denom, 1.0 / temperature, *numbers, kind, _DTYPES[x.dtype],
+            ids.dtype is torch.int64, 0 if teacher is None else ids.shape[-1],
+            0 if teacher is None else _DTYPES[teacher.dtype], x.device.index, 0)
+
+    def forward(self) -> None:
+        _launch("lz_loss_forward", self.args, _NAMES[self.args.kind])
+
+    def upstream(self, g, saved):
+        """(scalar upstream, upstream of each row's log-probability)."""
+        return (None, g) if self.args.kind == LOGP else (g, None)
+
+    def backward(self, saved, g) -> torch.Tensor:
+        """The gradient is handed out once: a second pass over a retained graph
+        writes into memory of its own."""
+        a, x, grad = self.args, saved[0], self.grad
+        if g.dtype is not torch.float32 or not g.is_contiguous():
+            g = g.to(torch.float32).contiguous()
+        if x.data_ptr() != a.logits:  # a saved tensor that came back from elsewhere
+            x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(x)
+            a.logits = x.data_ptr()
+        a.ids, a.work = saved[1].data_ptr(), saved[2].data_ptr()
+        if a.kind == DISTILL:
+            a.teacher = saved[3].data_ptr()
+        if grad is None:
+            a.fresh = 1
+            grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
+            a.grad = grad.data_ptr()
+        self.grad = None
+        scalar, rows = self.upstream(g, saved)
+        a.upstream, a.row_upstream = _ptr(scalar), _ptr(rows)
+        _launch("lz_loss_backward", a, _NAMES[a.kind])
+        return grad
 
 
 class _Loss(torch.autograd.Function):
-    """What the three losses and the log-probabilities share: the backward pass
-    is not differentiable itself, and says so where a graph of it is recorded."""
-
-    @classmethod
-    def backward(cls, ctx, g, *_):
-        if g is None:
-            return (None,) * ctx.inputs
-        if torch.is_grad_enabled():
-            return cls._recorded(ctx, g)
-        return (cls.gradient(ctx, g), *(None,) * (ctx.inputs - 1))
-
-    @classmethod
-    def _recorded(cls, ctx, g):
-        def gradient(ctx, g):
-            return cls.gradient(ctx, g)
-
-        return (torch.autograd.function.once_differentiable(gradient)(ctx, g), *(None,) * (ctx.inputs - 1))
-
-
-def _scalar_gradient(ctx, g):
-    """The gradient that the forward pass left, for upstream `g`. It is handed
-    out once: a second pass over a retained graph writes into memory of its own."""
-    x, ids, work, *teacher = ctx.saved_tensors
-    grad, ctx.grad = ctx.grad, None
-    return _finish(ctx.args, x, ids, work, ctx.shape, grad, _fp32(g), None, *teacher)
-
-
-def _run_token_logprobs(logits, tokens, temperature):
-    logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
-    return logp, *_start(LOGP, logits, tokens, temperature, out=(None, logp, None, None))
-
-
-class _TokenLogprobs(_Loss):
     @staticmethod
-    def forward(ctx, logits, tokens, temperature):
-        logp, ctx.args, x, work = _run_token_logprobs(logits, tokens, temperature)
-        ctx.save_for_backward(x, tokens, work)
-        ctx.shape, ctx.inputs = logits.shape, 3
-        return logp
+    def forward(ctx, logits, call):
+        call.forward()
+        ctx.save_for_backward(*call.keep)
+        ctx.call, out = call, call.out
+        call.keep = call.out = None  # the output leads here: it may not be held from here
+        return out
+
+    @staticmethod
+    def backward(ctx, g):
+        if torch.is_grad_enabled():  # a graph of the gradient is recorded: it may not be differentiated itself
+            return torch.autograd.function.once_differentiable(_Loss.gradient)(ctx, g), None
+        return _Loss.gradient(ctx, g), None
 
     @staticmethod
     def gradient(ctx, g):
-        x, ids, work = ctx.saved_tensors
-        return _finish(ctx.args, x, ids, work, ctx.shape, row_upstream=_fp32(g))
+        return ctx.call.backward(ctx.saved_tensors, g)
 
 
-def _run_policy(logits, tokens, rows, p, grad=None):
-    """rows: old_logp, advantages, ref_logp, weights; p: the loss's numbers."""
-    old = rows[0]  # contiguous, fp32, of the tokens' shape
-    out = (old.new_empty(()), torch.empty_like(old), None if rows[2] is None else torch.empty_like(old),
-           torch.empty_like(old, dtype=torch.bool))
-    return out, *_start(POLICY, logits, tokens, p["temperature"], p["denom"], grad, None, rows, out,
-                        (p["clip_low"], p["clip_high"], p["kl_coef"]))
+def _run(call: _Call, logits: torch.Tensor, needs_grad: bool) -> torch.Tensor:
+    if needs_grad:
+        return _Loss.apply(logits, call)
+    call.forward()
+    return call.out
 
 
-class _PolicyLoss(_Loss):
-    @staticmethod
-    def forward(ctx, logits, tokens, rows, p):
-        ctx.grad = _grad_like(logits)
-        out, ctx.args, x, work = _run_policy(logits, tokens, rows, p, ctx.grad)
-        ctx.save_for_backward(x, tokens, work)
-        ctx.mark_non_differentiable(*(t for t in out[1:] if t is not None))
-        ctx.set_materialize_grads(False)
-        ctx.shape, ctx.inputs = logits.shape, 4
-        return out
+class _PairsCall(_Call):
+    """The log-probabilities and, from them, the preference loss."""
 
-    gradient = staticmethod(_scalar_gradient)
+    def __init__(self, logits, tokens, ref, offsets, p):
+        dev, rows, pairs = logits.device, tokens.numel(), p["pairs"]
+        logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+        super().__init__(LOGP, logits, tokens, p["temperature"], logp, logp)
+        self.out = logp.new_empty(())
+        self.rewards = logp.new_empty(2 * pairs)
+        work = torch.empty(1 + pairs + (rows + 1) // 2, dtype=torch.float64, device=dev)
+        self.first = 1 + pairs  # of the rows' slopes in it
+        self.pairs = _PairArgs(
+            self.args.work, tokens.data_ptr(), _ptr(offsets), _ptr(ref), self.out.data_ptr(), self.rewards.data_ptr(),
+            work.data_ptr(), rows, pairs, p["length"], p["beta"], p["label_smoothing"], p["length_normalized"],
+            tokens.dtype is torch.int64, offsets is not None and offsets.dtype is torch.int64, dev.index)
+        self.alive = logp, ref, offsets
+        self.keep += (work,)
 
+    def forward(self) -> None:
+        super().forward()
+        _launch("lz_loss_pairs", self.pairs, "preference loss")
+        self.alive = None
 
-def _run_distill(logits, ids, teacher, weights, p, grad=None):
-    dev = logits.device
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    return (loss, kl), *_start(DISTILL, logits, ids, p["temperature"], p["denom"], grad, teacher,
-                               (None, None, None, weights), (loss, None, kl, None))
-
-
-class _DistillLoss(_Loss):
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, weights, p):
-        ctx.grad = _grad_like(logits)
-        out, ctx.args, x, work = _run_distill(logits, ids, teacher, weights, p, ctx.grad)
-        ctx.save_for_backward(x, ids, work, teacher)
-        ctx.mark_non_differentiable(out[1])
-        ctx.set_materialize_grads(False)
-        ctx.shape, ctx.inputs = logits.shape, 5
-        return out
-
-    gradient = staticmethod(_scalar_gradient)
-
-
-def _run_preference(logits, tokens, ref, offsets, p):
-    logp, args, x, work = _run_token_logprobs(logits, tokens, p["temperature"])
-    dev, pairs, rows = logits.device, p["pairs"], tokens.numel()
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    rewards = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
-    pair_work = torch.empty(1 + pairs + (rows + 1) // 2, dtype=torch.float64, device=dev)
-    a = _PairArgs(logp.data_ptr(), tokens.data_ptr(), _ptr(offsets), _ptr(ref), loss.data_ptr(), rewards.data_ptr(),
-                  pair_work.data_ptr(), rows, pairs, p["length"], p["beta"], p["label_smoothing"], p["length_normalized"],
-                  tokens.dtype is torch.int64, offsets is not None and offsets.dtype is torch.int64, dev.index)
-    _launch("lz_loss_pairs", a, "preference loss")
-    return loss, rewards, args, x, work, pair_work
-
-
-class _PreferenceLoss(_Loss):
-    @staticmethod
-    def forward(ctx, logits, tokens, ref, offsets, p):
-        loss, rewards, ctx.args, x, work, pair_work = _run_preference(logits, tokens, ref, offsets, p)
-        ctx.save_for_backward(x, tokens, work, pair_work)
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        ctx.shape, ctx.inputs, ctx.pairs = logits.shape, 5, p["pairs"]
-        return loss, rewards
-
-    @staticmethod
-    def gradient(ctx, g):
-        x, tokens, work, pair_work = ctx.saved_tensors
-        slope = pair_work[1 + ctx.pairs:].view(torch.float32)
-        return _finish(ctx.args, x, tokens, work, ctx.shape, upstream=_fp32(g), row_upstream=slope)
+    def upstream(self, g, saved):
+        return g, saved[3][self.first:]
 
 
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------
@@ -450,9 +399,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     temperature = _check_temperature(what, temperature)
     if not logits.is_cuda:
         return _cpu_token_logprobs(logits, tokens, temperature)
-    if _needs_grad(logits):
-        return _TokenLogprobs.apply(logits, tokens, temperature)
-    return _run_token_logprobs(logits, tokens, temperature)[0]
+    logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+    return _run(_Call(LOGP, logits, tokens, temperature, logp, logp), logits, _needs_grad(logits))
 
 
 @traced("policy_loss")
@@ -487,9 +435,12 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
          "temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
     if not logits.is_cuda:
         return PolicyLoss(*_cpu_policy_loss(logits, tokens, rows, p))
-    if _needs_grad(logits):
-        return PolicyLoss(*_PolicyLoss.apply(logits, tokens, rows, p))
-    return PolicyLoss(*_run_policy(logits, tokens, rows, p)[0])
+    needs_grad, old = _needs_grad(logits), rows[0]  # old_logp: contiguous, fp32, of the tokens' shape
+    logp, clipped = torch.empty_like(old), torch.empty_like(old, dtype=torch.bool)
+    kl = None if ref_logp is None else torch.empty_like(old)
+    call = _Call(POLICY, logits, tokens, p["temperature"], old.new_empty(()), logp, kl, clipped, rows, None, p["denom"],
+                 (p["clip_low"], p["clip_high"], p["kl_coef"]), needs_grad)
+    return PolicyLoss(_run(call, logits, needs_grad), logp, kl, clipped)
 
 
 @traced("preference_loss")
@@ -529,10 +480,9 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, *, ref_logp: tor
          "length_normalized": bool(length_normalized), "temperature": _check_temperature(what, temperature)}
     if not logits.is_cuda:
         loss, rewards = _cpu_preference_loss(logits, tokens, ref, cu_seqlens, p)
-    elif _needs_grad(logits):
-        loss, rewards = _PreferenceLoss.apply(logits, tokens, ref, cu_seqlens, p)
     else:
-        loss, rewards = _run_preference(logits, tokens, ref, cu_seqlens, p)[:2]
+        call = _PairsCall(logits, tokens, ref, cu_seqlens, p)
+        loss, rewards = _run(call, logits, _needs_grad(logits)), call.rewards
     return PreferenceLoss(loss, rewards[:p["pairs"]], rewards[p["pairs"]:])
 
 
@@ -568,6 +518,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     p = {"temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
     if not logits.is_cuda:
         return DistillLoss(*_cpu_distill_loss(logits, ids, teacher, weights, p))
-    if _needs_grad(logits):
-        return DistillLoss(*_DistillLoss.apply(logits, ids, teacher, weights, p))
-    return DistillLoss(*_run_distill(logits, ids, teacher, weights, p)[0])
+    needs_grad = _needs_grad(logits)
+    kl = torch.empty(shape, dtype=torch.float32, device=dev)
+    call = _Call(DISTILL, logits, ids, p["temperature"], kl.new_empty(()), None, kl, None, (None, None, None, weights), teacher,
+                 p["denom"], fused=needs_grad)
+    return DistillLoss(_run(call, logits, needs_grad), kl)

@@ -602,6 +602,31 @@ def test_captured_and_replayed(v):
     torch.cuda.synchronize()
 
 
+def test_a_dropped_graph_frees_its_memory():
+    """No cycle holds the gradient that the forward pass wrote, or the logits."""
+    import gc
+
+    x, y, old, adv, r = _policy_case(64, 40000, BF16, 2)
+    ids = y[:, None]
+    t = torch.zeros(64, 1, device="cuda")
+    gc.collect()
+    gc.disable()
+    try:
+        for f in (lambda z: lz.policy_loss(z, y, old, adv, ref_logp=r).loss, lambda z: lz.distill_loss(z, ids, t).loss,
+                  lambda z: lz.token_logprobs(z, y).sum(),
+                  lambda z: lz.preference_loss(z.view(2, 32, -1), y.view(2, 32)).loss):
+            before = torch.cuda.memory_allocated()
+            leaf = x.clone().requires_grad_(True)
+            loss = f(leaf)
+            del loss
+            loss = f(leaf)
+            g, = torch.autograd.grad(loss, leaf)
+            del loss, g, leaf
+            assert torch.cuda.memory_allocated() == before
+    finally:
+        gc.enable()
+
+
 def test_losses_under_autocast_and_checkpoint():
     from torch.utils.checkpoint import checkpoint
 
