@@ -4,6 +4,12 @@ step and pushes them to the inference ranks, which check what they received.
     torchrun --nproc-per-node 8 -m results_b200.examples.rl_weight_sync --steps 5
     torchrun --nproc-per-node 3 -m results_b200.examples.rl_weight_sync --device cpu --layers 2
 
+With ``--objective policy`` (or ``preference``, ``distill``) the update is a step of
+that loss on the output head instead of noise: every rank scores the step's rollout
+with the weights it holds (``token_logprobs``), the trainer checks that the inference
+ranks' log-probabilities are its own to the last bit, which is what a lossless sync
+is for, and learns from them.
+
 With ``--resume`` the trainer restarts from the newest dumped version
 (checkpoint / resume of the weight stream).
 
@@ -37,11 +43,55 @@ def checksum(sd) -> int:
     return s
 
 
+def rollout(sd, step: int, rows: int = 32):
+    """Hidden states and actions of a synthetic rollout, the same on every rank
+    that holds the same weights."""
+    g = torch.Generator().manual_seed(step)
+    emb, norm = sd["model.embed_tokens.weight"], sd["model.norm.weight"]
+    vocab = sd["lm_head.weight"].shape[0]
+    prompt = torch.randint(0, emb.shape[0], (rows,), generator=g).to(emb.device)
+    actions = torch.randint(0, vocab, (rows,), generator=g).to(emb.device)
+    return emb[prompt] * norm * emb.shape[1] ** 0.5, actions
+
+
+def score(sd, hidden, actions) -> torch.Tensor:
+    """Log-probabilities of a rollout's actions under the weights of this rank."""
+    from results_b200 import token_logprobs
+
+    with torch.no_grad():
+        return token_logprobs(hidden @ sd["lm_head.weight"].t(), actions)
+
+
+def objective_step(sd, objective: str, step: int, hidden, actions, old_logp):
+    """Loss of one step and its gradient in the output head."""
+    import results_b200 as lz
+
+    g = torch.Generator().manual_seed(1000 + step)
+    head = sd["lm_head.weight"].detach().clone().requires_grad_(True)
+    logits = hidden @ head.t()
+    rows = len(actions)
+    if objective == "policy":
+        advantages = torch.randn(rows, generator=g).to(logits.device)
+        loss = lz.policy_loss(logits, actions, old_logp, advantages, ref_logp=old_logp, kl_coef=0.05).loss
+    elif objective == "preference":  # the first half is preferred to the second, in answers of four tokens
+        loss = lz.preference_loss(logits.view(rows // 4, 4, -1), actions.view(rows // 4, 4),
+                                  ref_logp=old_logp.view(rows // 4, 4).sum(1)).loss
+    else:  # a teacher that is a little off the student
+        noise = torch.randn(logits.shape, generator=g).to(logits.device)
+        top = (logits.detach().float() + noise).topk(16)
+        loss = lz.distill_loss(logits, top.indices, top.values).loss
+    grad, = torch.autograd.grad(loss, head)
+    return loss.detach(), grad
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=3)
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--mode", default="raw", choices=["raw", "split_ans"])
+    ap.add_argument("--objective", default="noise", choices=["noise", "policy", "preference", "distill"],
+                    help="what the trainer's step is")
+    ap.add_argument("--lr", type=float, default=0.1, help="step size of --objective")
     ap.add_argument("--device", default="cuda", choices=["cuda", "cpu"])
     ap.add_argument("--symmetric", action="store_true", help="weights in the symmetric heap (zero-copy update)")
     ap.add_argument("--dump-dir", default=None)
@@ -90,11 +140,24 @@ def main(argv=None):
             start = v[0] + 1
     ok_all = True
     for step in range(start, start + a.steps):
-        if rank == 0:  # a synthetic optimizer step: every weight moves a little
+        note = ""
+        if a.objective != "noise" and (step > start or world == 1):  # from the second step on all ranks hold weights
+            hidden, actions = rollout(sd, step)
+            logp = score(sd, hidden, actions)
+            scores = [None] * world
+            dist.all_gather_object(scores, logp.cpu())
+            same = all(torch.equal(s, scores[0]) for s in scores)
+            ok_all = ok_all and same
+            if rank == 0:
+                loss, grad = objective_step(sd, a.objective, step, hidden, actions, logp)
+                sd["lm_head.weight"].sub_(a.lr * grad)
+                note = f", {a.objective} loss {float(loss):.4f}, log-probabilities equal on all ranks: {same}"
+        elif rank == 0:  # a synthetic optimizer step: every weight moves a little
             g = torch.Generator(device=dev).manual_seed(step)
             for t in sd.values():
                 if t.is_floating_point():
                     t.add_((torch.randn(t.shape, generator=g, device=dev) * 1e-3).to(t.dtype))
+        if rank == 0:
             if a.dump_dir and a.dump_every and step % a.dump_every == 0:
                 weights.dump_tensors(list(sd.items()), a.dump_dir, step, 0, group_name="trainer")
                 weights.mark_dump_complete(a.dump_dir, step, 1)
@@ -111,7 +174,7 @@ def main(argv=None):
         ok_all = ok_all and int(flag.item()) == 0
         if rank == 0:
             print(f"step {step}: weights v{step} on {world} ranks in {dt * 1e3:.1f} ms, "
-                  f"all receivers bit-exact: {int(flag.item()) == 0}", flush=True)
+                  f"all receivers bit-exact: {int(flag.item()) == 0}{note}", flush=True)
     if comm is not None:
         import results_b200 as lz
 
