@@ -39,8 +39,8 @@ struct LzLossArgs {
   float* logp;           // [rows] (LOGP, POLICY)
   float* kl;             // [rows] (POLICY with ref_logp, DISTILL)
   unsigned char* clipped;  // [rows] (POLICY)
-  // [HEAD + ROW rows], 16-byte aligned: head, then per row its normaliser (two
-  // doubles), the slope of the loss in its log-probability (LOGP: that itself, in
+  // [HEAD + ROW rows], 16-byte aligned: head, then per row its sum (four
+  // floats), the slope of the loss in its log-probability (LOGP: that itself, in
   // 64 bits, since sums of many are taken of it), its loss, and its
   // place in the order in which rows are taken (int)
   double* work;

@@ -107,6 +107,8 @@ def grad_off(ref, dtype, off, slope_off):
     p_off = p * (off[:, None] + 2.0 ** -21 + 2.0 ** -23 * (-p.clamp(min=1e-300).log2()))
     d = ref["slope"].abs()[:, None] * p_off + slope_off[:, None] * (ref["grad"] / torch.where(
         ref["slope"] == 0, 1.0, ref["slope"])[:, None]).abs() + 2.0 ** -22 * ref["grad"].abs()
-    # below the types' normal range: half a step of a subnormal, and exponentials under 2^-126 are zero
-    low = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -126 * ref["slope"].abs()[:, None]
+    # below the types' normal range: half a step of a subnormal, and exponentials under 2^-126 are zero.
+    # They count from an integer that is at most 1/2 above the row's maximum, so the sum that divides
+    # them is at least 2^-1/2 and what is lost at most 2^-125.5 of the slope
+    low = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -125.5 * ref["slope"].abs()[:, None]
     return d * (1 + half) + half * ref["grad"].abs() + low
