@@ -65,5 +65,6 @@ def __getattr__(name):
     if name in ("token_logprobs", "policy_loss", "preference_loss", "distill_loss"):
         from .ops import losses
 
-        return getattr(losses, name)
+        globals()[name] = fn = getattr(losses, name)  # small calls should not come through here again
+        return fn
     raise AttributeError(name)

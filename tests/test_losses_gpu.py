@@ -627,6 +627,56 @@ def test_a_dropped_graph_frees_its_memory():
         gc.enable()
 
 
+FIRST_CALL = r"""
+import torch
+import results_b200 as lz
+x = torch.randn(6, 50000, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+small = torch.randn(6, 500, device="cuda").requires_grad_(True)
+y = torch.arange(6, device="cuda")
+z = torch.zeros(6, device="cuda")
+out, g = [], torch.cuda.CUDAGraph()
+from results_b200 import _native
+_native.cuda()
+with torch.cuda.graph(g):
+    for t in (x, small):
+        out += torch.autograd.grad(lz.policy_loss(t, y, z - 9, z + 1).loss, t)
+        out += torch.autograd.grad(lz.token_logprobs(t, y), t, z + 1)
+g.replay()
+torch.cuda.synchronize()
+for i, t in enumerate((x, small)):
+    assert torch.equal(out[2 * i], torch.autograd.grad(lz.policy_loss(t, y, z - 9, z + 1).loss, t)[0])
+    assert torch.equal(out[2 * i + 1], torch.autograd.grad(lz.token_logprobs(t, y), t, z + 1)[0])
+print("captured first ok")
+"""
+
+
+def test_first_call_of_a_process_is_captured():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert "captured first ok" in r.stdout, r.stdout + r.stderr
+
+
+def test_many_rows_of_every_kind():
+    """More rows than teams and clusters, some of which do not count, at sizes where the kernels change."""
+    for n, v, dtype in ((9000, 700, BF16), (5000, 8000, FP16), (1300, 9001, FP32), (400, 30011, FP16), (311, 60000, BF16),
+                        (2500, 24000, BF16), (300, 33000, FP32), (700, 70000, BF16)):
+        case = _policy_case(n, v, dtype, n)
+        case[1][torch.rand(n, device="cuda", generator=_gen(1)) < 0.3] = -1
+        w = torch.rand(n, device="cuda", generator=_gen(2))
+        w[torch.rand(n, device="cuda", generator=_gen(3)) < 0.3] = 0
+        _check_policy(*case, w=w, upstream=1.0)
+        _check_policy(*case, w=w, upstream=-0.5)
+        x, ids, t = _distill_case(n, v, 33, dtype, n)
+        ids[::7, 5:] = -1
+        _check_distill(x, ids, t, w=w)
+        _check_distill(x, ids, t, w=w, upstream=2.0)
+        del case, x
+
+
 def test_losses_under_autocast_and_checkpoint():
     from torch.utils.checkpoint import checkpoint
 
