@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) row_kernel(const __grid
       __syncwarp();
     }
     RowSum n = {0.f, m, sum};
-    if (isinf(m)) n = slow_sum(x, a.vocab, c);
+    if (!exact_ref(m)) n = slow_sum(x, a.vocab, c);
     const RowOut o = row_out<KIND>(a, sh.params, n.norm(), c);
     const RowGrad g(o.slope, a.inv_temperature, n);
     if (GRAD) {

@@ -114,26 +114,6 @@ LZ_DEV uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// The largest element of a vector; NaN only if all are.
-template <typename T>
-LZ_DEV float vector_max(uint4 v);
-template <>
-LZ_DEV float vector_max<float>(uint4 v) {
-  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
-}
-template <>
-LZ_DEV float vector_max<__nv_bfloat16>(uint4 v) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-  return fmaxf(m.x, m.y);
-}
-template <>
-LZ_DEV float vector_max<__half>(uint4 v) {
-  const __half2* h = reinterpret_cast<const __half2*>(&v);
-  const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-  return fmaxf(m.x, m.y);
-}
-
 template <typename T>
 LZ_DEV void unpack_pairs(uint4 v, uint64_t* p) {
   float f[Elem<T>::N];
@@ -161,9 +141,9 @@ LZ_DEV long long single_of(int lead, int vecs, int per_vec, int t, long long n) 
   return t - lead < n - tail ? tail + t - lead : -1;
 }
 
-// p_j = 2^((x_j - base) c - lse2). base is 0 but in rows whose maximum times c
-// is beyond 32 bits (all of a row masked with the type's lowest value): there it
-// is that maximum, and the row takes the slow loops.
+// p_j = 2^((x_j - base) c - lse2). base is 0 but in rows whose maximum times c is
+// no integer's neighbour in fp32 any more (all of a row masked, with -1e10 or the
+// type's lowest value): there it is that maximum, and the row takes the slow loops.
 struct Norm {
   float base;
   double lse2;
@@ -215,6 +195,7 @@ LZ_DEV uint4 dense_vector(uint4 w, uint64_t c2, uint64_t neg_ref, uint64_t f2) {
 }
 
 constexpr int kBatch = 3;  // vectors a thread has in work at a time
+constexpr float kExactRef = 8388608.f;  // 2^23: references up to here are exact integers, and so is x c - ref near them
 
 // Sum over a thread's elements of 2^(x c - ref). ref is an integer, so that sums are
 // brought to another reference without a rounding (with the maximum itself as the
@@ -222,13 +203,14 @@ constexpr int kBatch = 3;  // vectors a thread has in work at a time
 // maximum: it is taken from the first batch and moves only when a batch's maximum is
 // more than 2^16 above it, which fp32 has room for (2^16 times the vocabulary), so
 // the exponentials of a batch wait for no maximum and the branch is seldom taken.
-// Rows of -inf sum to 0 with the reference -inf; a NaN or +inf makes the sum NaN.
+// A thread that sees nothing above -kExactRef / c leaves the reference -inf and a sum
+// of 0; a NaN or +inf makes the sum NaN.
 struct LazySum {
   float ref, limit;  // in units of x c, of x; ref is -inf (and taken as 0) before the first batch
   uint64_t neg_ref, sum[2];
   LZ_DEV void init(float c) {
     ref = -INFINITY, neg_ref = 0, sum[0] = sum[1] = 0;
-    limit = -3e38f / fmaxf(c, 1.f);  // below this x c is beyond 32 bits: such entries count nothing
+    limit = -kExactRef / c;  // entries below this count nothing beside 2^0
   }
   LZ_DEV float total() const {
     float s0, s1, s2, s3;
@@ -264,13 +246,30 @@ LZ_DEV void batch_sum(const uint4* w, uint64_t c2, uint64_t neg_ref, uint64_t* o
   }
 }
 
+// The largest element of U vectors; NaN only if all are.
+template <typename T, int U>
+LZ_DEV float batch_max(const uint4* w) {
+  if constexpr (sizeof(T) == 4) {
+    const float* f = reinterpret_cast<const float*>(w);
+    float m = f[0];
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = fmaxf(m, f[i]);
+    return m;
+  } else {
+    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    const T2* h = reinterpret_cast<const T2*>(w);
+    T2 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = __hmax2(m, h[i]);
+    return fmaxf(Elem<T>::get(m.x), Elem<T>::get(m.y));
+  }
+}
+
 // `first` (of a row): nothing to go by, so the maximum comes first.
 template <typename T, int U>
 LZ_DEV void take_batch(LazySum& s, const uint4* w, float c, bool first) {
   const uint64_t c2 = pair(c, c);
-  float m = vector_max<T>(w[0]);
-#pragma unroll
-  for (int u = 1; u < U; ++u) m = fmaxf(m, vector_max<T>(w[u]));
+  const float m = batch_max<T, U>(w);
   if (first && m > s.limit) s.raise(m, c);
   uint64_t part[2] = {0, 0};
   batch_sum<T, U>(w, c2, s.neg_ref, part);
@@ -295,7 +294,10 @@ LZ_DEV void lanes_join(float& m, float& s, int n) {
   m = top;
 }
 
-// Maximum and sum of a row whose scaled maximum is beyond 32 bits, by one warp.
+// Whether a joined reference is that of an ordinary row.
+LZ_DEV bool exact_ref(float ref) { return fabsf(ref) <= kExactRef; }
+
+// Maximum and sum of any other row, by one warp.
 template <typename T>
 LZ_DEV RowSum slow_sum(const T* x, long long n, float c) {
   const int lane = threadIdx.x % 32;
@@ -387,8 +389,7 @@ LZ_DEV RowOut row_out(const LzLossArgs& a, const RowParams& p, const Norm& n, fl
 }
 
 // Writes a row's outputs and what the backward pass takes (from which it gets the same
-// bits for upstream 1); returns its loss. `t`:
-// the teacher's list. One warp.
+// bits for upstream 1); returns its loss. `t`: the teacher's list. One warp.
 template <int KIND>
 LZ_DEV double row_outputs(const LzLossArgs& a, const RowParams& p, const RowOut& o, const RowSum& n, const TopView& t,
                           long long r, float c) {

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     LazySum sum;
     sum.init(c);
     int done = 0;  // chunks of the row that are in `sum`
-    // Chunks [done, upto) of a row, two at a time.
+    // Chunks [done, upto) of a row.
     auto take = [&](const RowHead& h, int upto) {
       for (; done < upto; ++done) {
         const int vecs = h.count - done * kChunkVecs;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         lanes_join(v.x, v.y, kMaxCluster);
       }
       RowSum n = {0.f, v.x, v.y};
-      if (isinf(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
+      if (!exact_ref(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
       if (KIND == LZ_LOSS_DISTILL) ring_wait<false>(&sh.ready[k], (turn >> 1) & 1, failed);
       const RowParams& p = sh.params[k];
       const RowOut o = row_out<KIND>(a, p, n.norm(), c);

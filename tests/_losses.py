@@ -93,7 +93,7 @@ def logp_off(logits, t, logp):
     log-probability by that share of the logits' spread, at most 2 max |z|;
     and the result is rounded."""
     z = logits.double().abs() / t
-    z = torch.where(z < 1e30, z, 0.0).amax(1)
+    z = torch.where(z < 1e6, z, 0.0).amax(1)  # beyond that entries are masked, or a row's own base is taken off first
     return 2.0 ** -24 * (logits.shape[1] / 256 + 64 + 4 + 1 + 2 * z * 1.45 + logp.abs())
 
 

@@ -311,6 +311,34 @@ def test_masked_vocabulary(dtype, v):
     _check_distill(x, ids, torch.zeros(8, 2, device="cuda"))
 
 
+@pytest.mark.parametrize("v", [40, 32003, 151552])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("mask", [-1e6, -1e9, -1e10, -1e20, -3e38])
+def test_large_masks(dtype, v, mask):
+    """Large finite masks: on half of a row, on all but one entry, on all of it; and rows that are that
+    large themselves. What is added to a mask is below its step, so masked entries are equal."""
+    x = _logits(8, v, dtype, 3)
+    mask = float(torch.tensor(mask, dtype=dtype))
+    x[0, : v // 2] = mask
+    x[1, v // 2:] = mask
+    x[2, :] = mask
+    x[2, v // 3] = 1.0
+    x[3, :] = mask
+    x[4, :] = -mask
+    x[5, 1:] = mask
+    x[6, :] = mask / 2
+    x[6, ::2] = mask
+    y = torch.tensor([v - 1, 0, v // 3, 1, 2, 0, 3, 4], device="cuda")
+    lp = oracle.logp64(x, y[:, None], 1.0)[0][:, 0]
+    adv = torch.ones(8, device="cuda")
+    # a row's own large values do not spread its probabilities: only differences from its maximum count
+    _check_policy(x, y, lp.float() - 0.1, adv, (lp - 0.2).float())
+    ids = torch.stack([y, (y + 7) % v], 1)
+    some = torch.tensor([0, 1, 3, 4, 7], device="cuda")  # rows whose list has no entry of probability zero
+    ids[:2, 1] = -1
+    _check_distill(x[some], ids[some], torch.zeros(5, 2, device="cuda"))
+
+
 @pytest.mark.parametrize("v", [17, 32003])
 def test_tokens_that_are_masked(v):
     """A token of probability zero: -inf as its log-probability, and the gradient's formula."""
