@@ -95,11 +95,9 @@ class DistillLoss(NamedTuple):
 def _check_logits(what: str, logits: torch.Tensor) -> None:
     if logits.dtype not in _DTYPES:
         raise TypeError(f"{what}: logits are {logits.dtype}; expected bfloat16, float16 or float32")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"{what}: logits of shape {tuple(logits.shape)} have no vocabulary")
-    if logits.shape[-1] > 2**31 - 1:
-        raise ValueError(f"{what}: a vocabulary of {logits.shape[-1]} entries is too large")
-    if logits.device.type not in ("cuda", "cpu"):
+    if not logits.dim() or not 0 < logits.shape[-1] < 2**31:
+        raise ValueError(f"{what}: logits of shape {tuple(logits.shape)}; expected a vocabulary of 1 to 2^31 - 1 entries")
+    if not (logits.is_cuda or logits.is_cpu):
         raise ValueError(f"{what}: device {logits.device} is not supported")
 
 
@@ -175,7 +173,7 @@ def _rows_of(x: torch.Tensor):
     v = x.shape[-1]
     if x.is_contiguous():
         rows = x.numel() // v
-        return x, 0, v, max(1, rows), rows
+        return x, 0, v, rows or 1, rows
     lead = x.shape[:-1]
     if x.stride(-1) != 1 and v > 1 or len(lead) > 2:
         return _rows_of(x.contiguous())
@@ -196,38 +194,47 @@ def _launch(fn: str, a, what: str) -> None:
         _native.check(rc, what)
 
 
-def _empty_grad(logits: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(logits, memory_format=torch.contiguous_format)
-
-
 class _Call:
     """One call: its arguments, its output `out`, and the tensors that the
     backward pass reads (`keep`, until autograd has them)."""
 
     def __init__(self, kind, logits, ids, temperature, out, logp=None, kl=None, clipped=None,
-                 rows=(None, None, None, None), teacher=None, denom=None, numbers=(0.0, 0.0, 0.0), fused=False):
+                 rows=None, teacher=None, denom=None, numbers=(0.0, 0.0, 0.0), fused=False):
         x, outer_stride, inner_stride, inner, n = _rows_of(logits)
-        work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=x.device)
+        dev = x.device
+        work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=dev)
         # the gradient for upstream 1, written by the forward pass
-        self.grad = _empty_grad(logits) if fused else None
+        self.grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if fused else None
         self.out, self.shape = out, logits.shape
         self.keep = (x, ids, work) if teacher is None else (x, ids, work, teacher)
+        a = self.args = _LossArgs(
+            x.data_ptr(), outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(self.grad), ids.data_ptr())
+        a.work, a.inv_temperature, a.kind = work.data_ptr(), 1.0 / temperature, kind
+        a.dtype, a.ids64, a.device = _DTYPES[x.dtype], ids.dtype is torch.int64, dev.index
+        a.logp = _ptr(logp)
+        if kind == LOGP:
+            return
         old, adv, ref, weights = rows
-        on_device = isinstance(denom, torch.Tensor)
-        self.args = _LossArgs(
-            x.data_ptr(), outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(self.grad), ids.data_ptr(), _ptr(teacher),
-            _ptr(old), _ptr(adv), _ptr(ref), _ptr(weights), denom.data_ptr() if on_device else None, None, None,
-            None if kind == LOGP else out.data_ptr(), _ptr(logp), _ptr(kl), _ptr(clipped), work.data_ptr(),
-            -1.0 if denom is None or on_device else denom, 1.0 / temperature, *numbers, kind, _DTYPES[x.dtype],
-            ids.dtype is torch.int64, 0 if teacher is None else ids.shape[-1],
-            0 if teacher is None else _DTYPES[teacher.dtype], x.device.index, 0)
+        a.loss, a.kl, a.clipped, a.weights = out.data_ptr(), _ptr(kl), _ptr(clipped), _ptr(weights)
+        if isinstance(denom, torch.Tensor):
+            a.denom_ptr = denom.data_ptr()
+        else:
+            a.denom = -1.0 if denom is None else denom
+        if kind == POLICY:
+            a.old_logp, a.advantages, a.ref_logp = old.data_ptr(), adv.data_ptr(), _ptr(ref)
+            a.clip_low, a.clip_high, a.kl_coef = numbers
+        else:
+            a.teacher, a.teacher_dtype, a.top = teacher.data_ptr(), _DTYPES[teacher.dtype], ids.shape[-1]
 
     def forward(self) -> None:
         _launch("lz_loss_forward", self.args, _NAMES[self.args.kind])
 
-    def upstream(self, g, saved):
-        """(scalar upstream, upstream of each row's log-probability)."""
-        return (None, g) if self.args.kind == LOGP else (g, None)
+    def set_upstream(self, g: int, saved) -> None:
+        """`g`: address of the upstream gradient, of each row's log-probability or of the loss."""
+        if self.args.kind == LOGP:
+            self.args.row_upstream = g
+        else:
+            self.args.upstream = g
 
     def backward(self, saved, g) -> torch.Tensor:
         """The gradient is handed out once: a second pass over a retained graph
@@ -246,8 +253,7 @@ class _Call:
             grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
             a.grad = grad.data_ptr()
         self.grad = None
-        scalar, rows = self.upstream(g, saved)
-        a.upstream, a.row_upstream = _ptr(scalar), _ptr(rows)
+        self.set_upstream(g.data_ptr(), saved)
         _launch("lz_loss_backward", a, _NAMES[a.kind])
         return grad
 
@@ -289,7 +295,7 @@ class _PairsCall(_Call):
         self.out = logp.new_empty(())
         self.rewards = logp.new_empty(2 * pairs)
         work = torch.empty(1 + pairs + (rows + 1) // 2, dtype=torch.float64, device=dev)
-        self.first = 1 + pairs  # of the rows' slopes in it
+        self.slopes = 8 * (1 + pairs)  # where the rows' slopes are in it, in bytes
         self.pairs = _PairArgs(
             self.args.work, tokens.data_ptr(), _ptr(offsets), _ptr(ref), self.out.data_ptr(), self.rewards.data_ptr(),
             work.data_ptr(), rows, pairs, p["length"], p["beta"], p["label_smoothing"], p["length_normalized"],
@@ -302,8 +308,8 @@ class _PairsCall(_Call):
         _launch("lz_loss_pairs", self.pairs, "preference loss")
         self.alive = None
 
-    def upstream(self, g, saved):
-        return g, saved[3][self.first:]
+    def set_upstream(self, g: int, saved) -> None:
+        self.args.upstream, self.args.row_upstream = g, saved[3].data_ptr() + self.slopes
 
 
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------
@@ -483,7 +489,7 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, *, ref_logp: tor
     else:
         call = _PairsCall(logits, tokens, ref, cu_seqlens, p)
         loss, rewards = _run(call, logits, _needs_grad(logits)), call.rewards
-    return PreferenceLoss(loss, rewards[:p["pairs"]], rewards[p["pairs"]:])
+    return PreferenceLoss(loss, *rewards.split(p["pairs"]))
 
 
 @traced("distill_loss")
