@@ -418,7 +418,13 @@ int run(const LzLossArgs* a, cudaStream_t s, bool forward) {
 
 extern "C" int lz_loss_forward(const LzLossArgs* a, cudaStream_t stream) { return run(a, stream, true); }
 
-extern "C" int lz_loss_backward(const LzLossArgs* a, cudaStream_t stream) { return run(a, stream, false); }
+extern "C" int lz_loss_backward(const LzLossArgs* a, cudaStream_t stream) {
+  // What only the forward pass reads may be gone by now.
+  LzLossArgs b = *a;
+  b.old_logp = b.advantages = b.ref_logp = b.weights = b.denom_ptr = nullptr;
+  b.loss = b.logp = b.kl = nullptr, b.clipped = nullptr;
+  return run(&b, stream, false);
+}
 
 extern "C" int lz_loss_pairs(const LzPairArgs* a, cudaStream_t stream) {
   if (a->pairs < 1 || a->pairs > INT32_MAX || a->rows < 0 || (!a->offsets && a->length * 2 * a->pairs != a->rows)) {

@@ -301,13 +301,17 @@ LZ_DEV bool exact_ref(float ref) { return fabsf(ref) <= kExactRef; }
 template <typename T>
 LZ_DEV RowSum slow_sum(const T* x, long long n, float c) {
   const int lane = threadIdx.x % 32;
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY, s = 0.f, part[8] = {};
 #pragma unroll 8
   for (long long i = lane; i < n; i += 32) m = fmaxf(m, Elem<T>::get(x[i]));
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-#pragma unroll 8
-  for (long long i = lane; i < n; i += 32) s += exp2_fast((Elem<T>::get(x[i]) - m) * c);
+  for (long long first = lane; first < n; first += 256)
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (first + 32 * u < n) part[u] += exp2_fast((Elem<T>::get(x[first + 32 * u]) - m) * c);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) s += part[u];
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   return {m, 0.f, s};

@@ -203,7 +203,7 @@ class _Call:
         x, outer_stride, inner_stride, inner, n = _rows_of(logits)
         dev = x.device
         work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=dev)
-        # the gradient for upstream 1, written by the forward pass
+        # the gradient for upstream 1, written by the forward pass; the first backward pass takes it away
         self.grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if fused else None
         self.out, self.shape = out, logits.shape
         self.keep = (x, ids, work) if teacher is None else (x, ids, work, teacher)
@@ -229,17 +229,18 @@ class _Call:
     def forward(self) -> None:
         _launch("lz_loss_forward", self.args, _NAMES[self.args.kind])
 
-    def set_upstream(self, g: int, saved) -> None:
+    def set_upstream(self, a, g: int, saved) -> None:
         """`g`: address of the upstream gradient, of each row's log-probability or of the loss."""
-        if self.args.kind == LOGP:
-            self.args.row_upstream = g
+        if a.kind == LOGP:
+            a.row_upstream = g
         else:
-            self.args.upstream = g
+            a.upstream = g
 
     def backward(self, saved, g) -> torch.Tensor:
         """The gradient is handed out once: a second pass over a retained graph
         writes into memory of its own."""
-        a, x, grad = self.args, saved[0], self.grad
+        a, x = _LossArgs.from_buffer_copy(self.args), saved[0]  # other threads may be here too
+        grad = self.__dict__.pop("grad", None)
         if g.dtype is not torch.float32 or not g.is_contiguous():
             g = g.to(torch.float32).contiguous()
         if x.data_ptr() != a.logits:  # a saved tensor that came back from elsewhere
@@ -252,8 +253,7 @@ class _Call:
             a.fresh = 1
             grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
             a.grad = grad.data_ptr()
-        self.grad = None
-        self.set_upstream(g.data_ptr(), saved)
+        self.set_upstream(a, g.data_ptr(), saved)
         _launch("lz_loss_backward", a, _NAMES[a.kind])
         return grad
 
@@ -308,8 +308,8 @@ class _PairsCall(_Call):
         _launch("lz_loss_pairs", self.pairs, "preference loss")
         self.alive = None
 
-    def set_upstream(self, g: int, saved) -> None:
-        self.args.upstream, self.args.row_upstream = g, saved[3].data_ptr() + self.slopes
+    def set_upstream(self, a, g: int, saved) -> None:
+        a.upstream, a.row_upstream = g, saved[3].data_ptr() + self.slopes
 
 
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------

@@ -495,6 +495,53 @@ def test_backward_twice_and_leaves():
         loss.backward()
 
 
+@pytest.mark.parametrize("v", [700, 40000])
+def test_what_the_forward_pass_alone_read_may_be_gone(v):
+    """The backward pass for another upstream, after the forward pass's weights (converted copies
+    here) and scores have been freed and their memory given back."""
+    case = _policy_case(12, v, BF16, 3)
+    x, ids, t = _distill_case(12, v, 9, BF16, 4)
+    mask = torch.rand(12, device="cuda", generator=_gen(1)) < 0.7
+    want = [_check_policy(*case, w=mask, upstream=2.0)[1], _check_distill(x, ids, t, w=mask, upstream=2.0)[1]]
+    leaves = [case[0].detach().requires_grad_(True), x.detach().requires_grad_(True)]
+    losses = [lz.policy_loss(leaves[0], case[1], case[2].clone(), case[3].clone(), ref_logp=case[4].clone(), weights=mask.clone(),
+                             clip_low=0.2, clip_high=0.25, kl_coef=0.1).loss,
+              lz.distill_loss(leaves[1], ids.clone(), t.clone(), weights=mask.clone()).loss]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    for loss, leaf, g in zip(losses, leaves, want):
+        assert torch.equal(torch.autograd.grad(loss * 2, leaf)[0], g)
+
+
+def test_two_threads_on_one_graph():
+    import threading
+
+    x, y, old, adv, r = _policy_case(40, 9000, BF16, 2)
+    x.requires_grad_(True)
+    loss = lz.policy_loss(x, y, old, adv, ref_logp=r, kl_coef=0.1).loss
+    want, = torch.autograd.grad(lz.policy_loss(x, y, old, adv, ref_logp=r, kl_coef=0.1).loss * 3, x)
+    one, = torch.autograd.grad(lz.policy_loss(x, y, old, adv, ref_logp=r, kl_coef=0.1).loss, x)
+    got, errors = [None] * 8, []
+
+    def work(k):
+        try:
+            up = torch.tensor(3.0 if k % 2 else 1.0, device="cuda")
+            got[k], = torch.autograd.grad(loss, x, up, retain_graph=True)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for k in range(8):
+        assert torch.equal(got[k], want if k % 2 else one)
+    assert len({g.data_ptr() for g in got}) == 8
+
+
 def test_no_second_derivatives():
     """A graph of the gradient may be recorded; to differentiate it is refused."""
     x, y, old, adv, r = _policy_case(6, 300, FP32, 2)
