@@ -25,11 +25,10 @@ LZ_DEV V block_sum(V v, V* red, int warps) {
 // ---- rows that a team of TEAM threads does alone: a warp where a row is small
 // (nothing waits for a barrier), a block otherwise. ----
 
-// One thread's share of a row's sum.
+// Thread `tid`'s share of a row's sum among TEAM.
 template <typename T, int TEAM>
-LZ_DEV LazySum row_sum(const T* x, long long n, float c) {
+LZ_DEV LazySum row_sum(const T* x, long long n, float c, int tid) {
   constexpr int U = 4;
-  const int tid = threadIdx.x % TEAM;
   LazySum s;
   s.init(c);
   const Split<T> sp(x, n);
@@ -136,9 +135,13 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) row_kernel(const __grid
       if (GRAD) row_dense<T, TEAM>(x, out, a.vocab, RowGrad(0.f, 1.f, RowSum{0.f, 0.f, 1.f}), c);
       continue;
     }
+    // A block's first warp has the teacher's list while the others have the row; a token's scalars are
+    // fetched behind the row, when its logit is in the caches.
+    constexpr int kSkip = KIND == LZ_LOSS_DISTILL && TEAM > 32 ? 32 : 0;
+    LazySum s;
+    s.init(c);
     if (KIND == LZ_LOSS_DISTILL && warp == 0) prepare_params<T, KIND>(a, x, r, sh.params, list, table, hash, c);
-    const LazySum s = row_sum<T, TEAM>(x, a.vocab, c);
-    // a token's scalars are fetched behind the row: its logit is in the caches by now
+    if (tid >= kSkip) s = row_sum<T, TEAM - kSkip>(x, a.vocab, c, tid - kSkip);
     if (KIND != LZ_LOSS_DISTILL && warp == 0) prepare_params<T, KIND>(a, x, r, sh.params, list, table, hash, c);
     float m = s.ref, sum = s.total();
     lanes_join(m, sum, 32);
