@@ -6,9 +6,11 @@ namespace {
 
 constexpr int kThreads = 512;  // of head_kernel and pair_kernel
 constexpr int kWarps = kThreads / 32;
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kRowCtas = 4;  // an SM: 64 registers a thread
+// CTAs an SM: 64 registers a thread. With four blocks of 256 the sums of 8192 rows of
+// 64 KB took 110 us, not 96.
+constexpr int kRowCtas = 8;
 
 template <typename V>
 LZ_DEV V block_sum(V v, V* red, int warps) {
@@ -328,9 +330,9 @@ struct OnDevice {
 };
 
 // The rows' grid, a team a row at a time, and the team's lists. A warp where rows are
-// many and short, or tiny; in us, bf16, warp against block, policy with its gradient:
-// 8192 rows of 16 KB 91 / 121, of 32 KB 163 / 165 (sums only 53 / 82), of 64 KB 302 /
-// 259; 1024 rows of 32 KB 38 / 32; 128 rows of 16 KB 26 / 16.
+// very many and short, or tiny; in us, bf16, warp against block, policy with its
+// gradient: 8192 rows of 8 KB 53 / 67, of 16 KB 90 / 91 (sums only 31 / 41), of 32 KB
+// 161 / 140; 1024 rows of 8 KB 20 / 18, of 16 KB 25 / 21; 128 rows of 16 KB 26 / 17.
 struct RowLaunch {
   int team, grid, hash;
   size_t smem;
@@ -344,7 +346,7 @@ int plan_rows(const LzLossArgs* a, RowLaunch* l) {
   l->hash = 0;
   if (distill && a->top > kSmallList)
     for (l->hash = 32; l->hash < 2 * a->top;) l->hash *= 2;
-  const bool warp = row <= 2048 || (row <= 16384 && a->rows >= 6ll * sms) || (row <= 32768 && a->rows >= 32ll * sms);
+  const bool warp = row <= 2048 || (row <= 16384 && a->rows >= 32ll * sms);
   l->team = warp && (!distill || a->top <= kSmallList) ? 32 : kRowThreads;
   const int teams = kRowThreads / l->team;
   const long long ctas = (a->rows + teams - 1) / teams, cap = (long long)sms * kRowCtas;

@@ -587,9 +587,9 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
 // offset from a 16-byte border. A row costs a cluster some 5000 cycles besides its
 // bytes (DISTILL's list 10000), which the many teams of row_kernel hide better
 // while rows are short; it reads a row that outgrows the caches a second time. In
-// us, bf16, streamed against teams: 8192 rows of 64 KB, sums only 130 / 113, of
-// 300 KB 360 / 630; with the policy's gradient 32 KB 171 / 165, 64 KB 210 / 259;
-// with DISTILL's of 64 entries 64 KB 371 / 292, 100 KB 394 / 455; the gradient
+// us, bf16, streamed against teams: 8192 rows of 64 KB, sums only 130 / 96, 4096 of
+// 300 KB 194 / 204; 8192 with the policy's gradient 32 KB 171 / 140, 64 KB 208 / 259;
+// with DISTILL's of 64 entries 64 KB 371 / 286, 100 KB 394 / 464; the gradient
 // alone, 1024 rows of 64 KB 25 / 21, 8192 rows of 100 KB 256 / 266. Few rows are
 // streamed whatever their length, since a cluster splits them.
 template <typename T>
