@@ -1,5 +1,7 @@
 // Vocabulary losses: entry points, and rows that a team of threads does alone
 // (small vocabularies; rows that cannot be streamed, see lz_losses_stream.cu).
+#include <algorithm>
+
 #include "lz_losses_dev.cuh"
 
 namespace {
@@ -11,6 +13,8 @@ constexpr int kRowWarps = kRowThreads / 32;
 // CTAs an SM: 64 registers a thread. With four blocks of 256 the sums of 8192 rows of
 // 64 KB took 110 us, not 96.
 constexpr int kRowCtas = 8;
+constexpr long long kWarpBytes = 8192;  // of the rows that a warp has at a time
+constexpr long long kHeadRows = 2048;   // more are the head's cluster's
 
 template <typename V>
 LZ_DEV V block_sum(V v, V* red, int warps) {
@@ -46,8 +50,11 @@ LZ_DEV LazySum row_sum(const T* x, long long n, float c, int tid) {
     const uint4 w = __ldg(v + i);
     take_batch<T, 1>(s, &w, c, true);
   }
-  const long long single = tid < 2 * Elem<T>::N ? single_of(sp.lead, sp.vecs, Elem<T>::N, tid, n) : -1;
-  if (single >= 0) s.take_one(Elem<T>::get(x[single]), c);
+#pragma unroll
+  for (int t = tid; t < 2 * Elem<T>::N; t += TEAM) {
+    const long long single = single_of(sp.lead, sp.vecs, Elem<T>::N, t, n);
+    if (single >= 0) s.take_one(Elem<T>::get(x[single]), c);
+  }
   return s;
 }
 
@@ -76,8 +83,11 @@ LZ_DEV void row_dense(const T* x, T* out, long long n, const RowGrad& g, float c
       if (i + u * TEAM < sp.vecs)
         st_cs_v4(o + i + u * TEAM, g.f == 0.f ? make_uint4(0, 0, 0, 0) : dense_vector<T>(w[u], c2, neg_ref, f2));
   }
-  const long long single = tid < 2 * N ? single_of(sp.lead, sp.vecs, N, tid, n) : -1;
-  if (single >= 0) out[single] = Elem<T>::put(g.f == 0.f ? 0.f : g.dense(Elem<T>::get(x[single]), c));
+#pragma unroll
+  for (int t = tid; t < 2 * N; t += TEAM) {
+    const long long single = single_of(sp.lead, sp.vecs, N, t, n);
+    if (single >= 0) out[single] = Elem<T>::put(g.f == 0.f ? 0.f : g.dense(Elem<T>::get(x[single]), c));
+  }
 }
 
 // The entries with t_j != 0, over what row_dense wrote (by all of the team, before). One warp.
@@ -103,6 +113,7 @@ LZ_DEV void team_sync() {
 struct TeamShared {
   RowParams params;
   float2 part[kRowWarps];
+  double loss;
 };
 
 template <int TEAM>
@@ -112,17 +123,34 @@ LZ_DEV TopView team_list(char* dynamic, int team, int top, int hash, int** table
   return TopView{reinterpret_cast<int*>(f), f + top, f + 2 * top, f + 3 * top};
 }
 
+// The CTA that is done last adds the CTAs' losses (`loss`, in thread 0) up, in their order.
+LZ_DEV void finish_loss(const LzLossArgs& a, double loss) {
+  __shared__ double red[kRowWarps];
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    work_loss(a)[blockIdx.x] = loss;
+    __threadfence();
+    last = atomicAdd(work_ticket(a), 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0.0;
+  for (unsigned k = threadIdx.x; k < gridDim.x; k += kRowThreads) s += __ldcg(work_loss(a) + k);
+  s = block_sum(s, red, kRowWarps);
+  if (threadIdx.x == 0) *a.loss = (float)s;
+}
+
 // The sum of a row, its scalars and outputs, then the gradient from a second look
 // at the row, which the caches still hold.
 template <typename T, int KIND, bool GRAD, int TEAM>
 __global__ void __launch_bounds__(kRowThreads, kRowCtas) row_kernel(const __grid_constant__ LzLossArgs a, int hash) {
   constexpr int kTeams = kRowThreads / TEAM;
   __shared__ TeamShared teams[kTeams];
-  __shared__ double red[kRowWarps];
-  __shared__ bool last;
   extern __shared__ __align__(16) char dynamic[];
   const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, warp = tid / 32, lane = tid % 32;
   TeamShared& sh = teams[team];
+  if (tid == 0) sh.loss = 0.0;
   int* table = nullptr;
   const TopView list = team_list<TEAM>(dynamic, team, KIND == LZ_LOSS_DISTILL ? a.top : 0, hash, &table);
   const float c = (float)(kLog2e * (double)a.inv_temperature);
@@ -130,10 +158,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) row_kernel(const __grid
     T* out = static_cast<T*>(a.grad) + (GRAD ? r * a.vocab : 0);
     const T* x = row_of<T>(a, r);
     if (!row_counts<KIND>(a, r)) {
-      if (tid == 0) {
-        no_outputs<KIND>(a, r);
-        if (KIND != LZ_LOSS_LOGP) work_loss(a)[r] = 0.0;
-      }
+      if (tid == 0) no_outputs<KIND>(a, r);
       if (GRAD) row_dense<T, TEAM>(x, out, a.vocab, RowGrad(0.f, 1.f, RowSum{0.f, 0.f, 1.f}), c);
       continue;
     }
@@ -167,22 +192,113 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) row_kernel(const __grid
     }
     if (warp == 0) {
       const double loss = row_outputs<KIND>(a, sh.params, o, n, list, r, c);
-      if (KIND != LZ_LOSS_LOGP && lane == 0) work_loss(a)[r] = loss;
+      if (KIND != LZ_LOSS_LOGP && lane == 0) sh.loss += loss;
     }
     team_sync<TEAM>();  // the next row's scalars and list overwrite this one's
   }
   if (KIND == LZ_LOSS_LOGP) return;
-  // The CTA that is done last adds the rows' losses up, in the rows' order.
-  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(work_ticket(a), 1u) == gridDim.x - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
   double s = 0.0;
-  for (long long r = threadIdx.x; r < a.rows; r += kRowThreads) s += __ldcg(work_loss(a) + r);
-  s = block_sum(s, red, kRowWarps);
-  if (threadIdx.x == 0) *a.loss = (float)s;
+  for (int k = 0; k < kTeams; ++k) s += teams[k].loss;
+  finish_loss(a, s);
+}
+
+// LOGP and POLICY, short rows where they are very many: `batch` of them a warp at a
+// time, L lanes a row, and the scalars and outputs of each by a lane of its own. A warp
+// a row spends more instructions on what is per row than on its elements.
+
+// (reference, sum) over L lanes, as lanes_join.
+template <int L>
+LZ_DEV void group_join(float& m, float& s) {
+  float top = m;
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  s *= m == -INFINITY ? 1.f : exp2_fast(m - top);  // a sum without a reference is 0 or NaN
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  m = top;
+}
+
+// The gradients of the rows from `first` on; `g`, `token` and `xy` are those of the lane's row.
+template <typename T, int L>
+LZ_DEV void warp_gradients(const LzLossArgs& a, long long first, int rows, const RowGrad& g, int token, float xy, float c) {
+  const int lane = threadIdx.x % 32;
+  T* out = static_cast<T*>(a.grad) + first * a.vocab;
+  for (int j = 0; j < rows; j += 32 / L) {
+    const int i = j + lane / L;
+    RowGrad d;
+    d.f = __shfl_sync(~0u, g.f, i), d.base = __shfl_sync(~0u, g.base, i), d.ref = __shfl_sync(~0u, g.ref, i);
+    if (i < rows) row_dense<T, L>(row_of<T>(a, first + i), out + i * a.vocab, a.vocab, d, c);
+  }
+  __syncwarp();
+  if (lane < rows && g.f != 0.f && token >= 0) out[lane * a.vocab + token] = Elem<T>::put(g.sparse(xy, 1.f, c));
+}
+
+template <typename T, int KIND, bool GRAD, int L>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas) warp_kernel(const __grid_constant__ LzLossArgs a, int batch) {
+  __shared__ double red[kRowWarps];
+  const int lane = threadIdx.x % 32;
+  const float c = (float)(kLog2e * (double)a.inv_temperature);
+  const long long at = ((long long)blockIdx.x * kRowWarps + threadIdx.x / 32) * batch, step = (long long)gridDim.x * kRowWarps * batch;
+  double loss = 0.0;
+  for (long long first = at; first < a.rows; first += step) {
+    const long long r = first + lane;
+    const int rows = (int)min((long long)batch, a.rows - first);
+    const bool counts = lane < rows && row_counts<KIND>(a, r);
+    const unsigned counted = __ballot_sync(~0u, counts);
+    RowSum n = {0.f, 0.f, 1.f};
+    for (int j = 0; j < rows; j += 32 / L) {
+      const int i = j + lane / L;
+      LazySum s;
+      s.init(c);
+      if (counted >> i & 1) s = row_sum<T, L>(row_of<T>(a, first + i), a.vocab, c, lane % L);
+      float m = s.ref, sum = s.total();
+      group_join<L>(m, sum);
+      m = __shfl_sync(~0u, m, lane % (32 / L) * L), sum = __shfl_sync(~0u, sum, lane % (32 / L) * L);
+      if (lane / (32 / L) == j / (32 / L)) n.ref = m, n.sum = sum;
+    }
+    for (unsigned odd = __ballot_sync(~0u, counts && !exact_ref(n.ref)); odd; odd &= odd - 1) {
+      const int i = __ffs(odd) - 1;
+      const RowSum v = slow_sum(row_of<T>(a, first + i), a.vocab, c);
+      if (lane == i) n = v;
+    }
+    RowParams p;
+    p.token = -1, p.xy = 0.f;
+    RowGrad g(0.f, 1.f, RowSum{0.f, 0.f, 1.f});
+    if (counts) {
+      token_params<T, KIND>(a, row_of<T>(a, r), r, p);
+      const RowOut o = row_out<KIND>(a, p, n.norm(), c);
+      g = RowGrad(o.slope, a.inv_temperature, n);
+      loss += row_write<KIND>(a, p, o, n, 0.0, r, true);
+    } else if (lane < rows) {
+      no_outputs<KIND>(a, r);
+    }
+    if (GRAD) warp_gradients<T, L>(a, first, rows, g, p.token, p.xy, c);
+  }
+  if (KIND != LZ_LOSS_LOGP) finish_loss(a, block_sum(loss, red, kRowWarps));
+}
+
+template <typename T, int KIND, int L>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas) warp_grad_kernel(const __grid_constant__ LzLossArgs a, int batch) {
+  const float up = a.upstream ? *a.upstream : 1.f;
+  if (!a.fresh && up == 1.f) return;
+  const int lane = threadIdx.x % 32;
+  const float c = (float)(kLog2e * (double)a.inv_temperature);
+  const long long at = ((long long)blockIdx.x * kRowWarps + threadIdx.x / 32) * batch, step = (long long)gridDim.x * kRowWarps * batch;
+  for (long long first = at; first < a.rows; first += step) {
+    const long long r = first + lane;
+    const int rows = (int)min((long long)batch, a.rows - first);
+    RowGrad g(0.f, 1.f, RowSum{0.f, 0.f, 1.f});
+    int token = -1;
+    float xy = 0.f;
+    if (lane < rows) {
+      const float4 sum = work_sum(a)[r];
+      const long long y = load_id(a.ids, a.ids64, r);
+      g = RowGrad((float)row_slope_for<KIND>(a, r, y, up), a.inv_temperature, RowSum{sum.x, sum.y, sum.z});
+      if (g.f != 0.f && y < a.vocab) token = (int)y, xy = Elem<T>::get(row_of<T>(a, r)[y]);
+    }
+    warp_gradients<T, L>(a, first, rows, g, token, xy, c);
+  }
 }
 
 // The gradient from the rows' saved sums and slopes. POLICY and DISTILL: where
@@ -223,48 +339,80 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) row_grad_kernel(const _
 // 1 / denominator (0 where that is not positive: nothing counts), the ticket and,
 // where `order` is set, the rows that count in front of those that do not, each
 // in their order: taken in turns, every cluster of the streamed kernel gets as many.
+// A cluster of CTAs where rows are many, each with a part of them: 8192 rows take 7 us, by
+// one CTA 13, 262144 rows 19, by one CTA 80.
+struct HeadPart {
+  double weights;
+  long long rows;  // that count
+};
+
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) head_kernel(const __grid_constant__ LzLossArgs a, bool order) {
   __shared__ double red[kWarps];
+  __shared__ long long red_rows[kWarps];
   __shared__ int counts[2][kWarps];
+  __shared__ alignas(16) HeadPart part;
+  constexpr int U = 8;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  double s = 0.0;
-  if (KIND != LZ_LOSS_LOGP) {
-    if (a.denom_ptr) {
-      s = (double)*a.denom_ptr;
-    } else if (a.denom >= 0.0) {
-      s = a.denom;
-    } else {
-      for (long long r = threadIdx.x; r < a.rows; r += kThreads)
-        if (KIND == LZ_LOSS_DISTILL || load_id(a.ids, a.ids64, r) >= 0) s += a.weights ? (double)a.weights[r] : 1.0;
-      s = block_sum(s, red, kWarps);
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const long long per = (a.rows + ranks - 1) / ranks, begin = min(rank * per, a.rows), end = min(begin + per, a.rows);
+  const bool given = KIND == LZ_LOSS_LOGP || a.denom_ptr || a.denom >= 0.0;
+  HeadPart all = {0.0, 0};
+  long long before = 0;  // rows of the ranks before this that count
+  if (!given || (order && ranks > 1)) {
+    for (long long first = begin + threadIdx.x; first < end; first += U * kThreads) {
+      long long id[U];
+      float w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // no branch: the loads run together
+        const long long r = min(first + u * kThreads, end - 1);
+        id[u] = KIND == LZ_LOSS_DISTILL ? 0 : load_id(a.ids, a.ids64, r);
+        w[u] = KIND != LZ_LOSS_LOGP && a.weights ? a.weights[r] : 1.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (id[u] >= 0 && first + u * kThreads < end) all.weights += (double)w[u], all.rows += w[u] != 0.f;
+    }
+    all.weights = block_sum(all.weights, red, kWarps);
+    if (ranks > 1) {
+      all.rows = block_sum(all.rows, red_rows, kWarps);
+      if (threadIdx.x == 0) part = all;
+      cluster_sync();
+      all = {0.0, 0};
+      for (uint32_t k = 0; k < ranks; ++k) {
+        const HeadPart v = peer_value(&part, k);
+        all.weights += v.weights, all.rows += v.rows;
+        if (k < rank) before += v.rows;
+      }
+      cluster_sync();  // no CTA leaves while a peer reads its part
     }
   }
-  if (threadIdx.x == 0) {
+  if (rank == 0 && threadIdx.x == 0) {
+    const double s = given ? (a.denom_ptr ? (double)*a.denom_ptr : a.denom) : all.weights;
     a.work[0] = s > 0.0 || s != s ? 1.0 / s : 0.0;
     *work_ticket(a) = 0u;
     if (KIND != LZ_LOSS_LOGP && a.rows == 0) *a.loss = 0.f;
   }
   if (!order) return;
   const int n = (int)a.rows;
-  int front = 0, back = 0;  // rows placed at either end
-  for (int first = 0, k = 0; first < n; first += kThreads, k ^= 1) {
+  int front = (int)before, back = (int)(begin - before);  // rows placed at either end
+  for (int first = (int)begin, k = 0; first < end; first += kThreads, k ^= 1) {
     const int r = first + threadIdx.x;
-    const bool counts_ = r < n && row_counts<KIND>(a, r);
+    const bool counts_ = r < end && row_counts<KIND>(a, r);
     const unsigned m = __ballot_sync(~0u, counts_);
     if (lane == 0) counts[k][warp] = __popc(m);
     __syncthreads();
-    int before = 0, all = 0;
+    int ahead = 0, here = 0;
     for (int w = 0; w < kWarps; ++w) {
-      before += w < warp ? counts[k][w] : 0;
-      all += counts[k][w];
+      ahead += w < warp ? counts[k][w] : 0;
+      here += counts[k][w];
     }
-    before += __popc(m & ((1u << lane) - 1));
-    if (r < n) work_order(a)[counts_ ? front + before : n - 1 - (back + (int)threadIdx.x - before)] = r;
-    front += all;
-    back += min(kThreads, n - first) - all;
+    ahead += __popc(m & ((1u << lane) - 1));
+    if (r < end) work_order(a)[counts_ ? front + ahead : n - 1 - (back + (int)threadIdx.x - ahead)] = r;
+    front += here;
+    back += min(kThreads, (int)end - first) - here;
   }
-  if (threadIdx.x == 0) *work_active(a) = front;
+  if (rank == ranks - 1 && threadIdx.x == 0) *work_active(a) = front;
 }
 
 // Preference loss of one pair a CTA: sums of its two sequences' log-probabilities
@@ -329,12 +477,15 @@ struct OnDevice {
   }
 };
 
-// The rows' grid, a team a row at a time, and the team's lists. A warp where rows are
-// very many and short, or tiny; in us, bf16, warp against block, policy with its
-// gradient: 8192 rows of 8 KB 53 / 67, of 16 KB 90 / 91 (sums only 31 / 41), of 32 KB
-// 161 / 140; 1024 rows of 8 KB 20 / 18, of 16 KB 25 / 21; 128 rows of 16 KB 26 / 17.
+// The rows' grid, a team a row at a time, and the team's lists. A warp or a part of
+// one where rows are very many and short, a warp where they are tiny. In us, bf16, a
+// part against a warp, policy with its gradient: 262144 rows of 512 bytes 114 / 417 (sums
+// only 37 / 116), 32768 rows of 2 KB 57 / 88, of 4 KB 93 / 111, 8192 rows of 4 KB 33 / 36. A
+// warp against a block: 8192 rows of 8 KB 53 / 67, of 16 KB 90 / 91 (sums only 31 / 41), of
+// 32 KB 161 / 140; 1024 rows of 8 KB 20 / 18, of 16 KB 25 / 21; 128 rows of 16 KB 26 / 17.
 struct RowLaunch {
   int team, grid, hash;
+  int batch;  // rows that a warp has at a time
   size_t smem;
 };
 
@@ -343,22 +494,44 @@ int plan_rows(const LzLossArgs* a, RowLaunch* l) {
   LZ_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, a->device));
   const bool distill = a->kind == LZ_LOSS_DISTILL;
   const long long row = a->vocab * (a->dtype == LZ_F32 ? 4 : 2);
+  const long long cap = (long long)sms * kRowCtas, each = (a->rows + cap * kRowWarps - 1) / (cap * kRowWarps);  // rows a warp
   l->hash = 0;
   if (distill && a->top > kSmallList)
     for (l->hash = 32; l->hash < 2 * a->top;) l->hash *= 2;
   const bool warp = row <= 2048 || (row <= 16384 && a->rows >= 32ll * sms);
   l->team = warp && (!distill || a->top <= kSmallList) ? 32 : kRowThreads;
-  const int teams = kRowThreads / l->team;
-  const long long ctas = (a->rows + teams - 1) / teams, cap = (long long)sms * kRowCtas;
-  l->grid = (int)(ctas < cap ? ctas : cap);
+  if (!distill && row <= 2048 && each >= 4) l->team = 8;
+  else if (!distill && row <= 4096 && each >= 2) l->team = 16;
+  const int teams = kRowThreads / l->team, at_once = l->team < 32 ? 32 / l->team : 1;
+  // All warps' batches together stay in L2 until their gradient.
+  l->batch = l->team < 32 ? (int)std::max((long long)at_once, std::min({32ll, each, kWarpBytes / row})) : 1;
   l->smem = distill ? (size_t)teams * (4 * a->top + l->hash) * 4 : 0;
+  const int of_cta = l->team < 32 ? kRowWarps * l->batch : teams;
+  const long long ctas = (a->rows + of_cta - 1) / of_cta;
+  l->grid = (int)(ctas < cap ? ctas : cap);
   return LZE_OK;
 }
 
 template <typename T, int KIND, bool GRAD>
 void launch_rows(const LzLossArgs* a, const RowLaunch& l, cudaStream_t s) {
+  if constexpr (KIND != LZ_LOSS_DISTILL)
+    switch (l.team) {
+      case 8: return warp_kernel<T, KIND, GRAD, 8><<<l.grid, kRowThreads, 0, s>>>(*a, l.batch);
+      case 16: return warp_kernel<T, KIND, GRAD, 16><<<l.grid, kRowThreads, 0, s>>>(*a, l.batch);
+    }
   if (l.team == 32) row_kernel<T, KIND, GRAD, 32><<<l.grid, kRowThreads, l.smem, s>>>(*a, l.hash);
   else row_kernel<T, KIND, GRAD, kRowThreads><<<l.grid, kRowThreads, l.smem, s>>>(*a, l.hash);
+}
+
+template <int KIND>
+int launch_head(const LzLossArgs* a, bool order, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {a->rows > kHeadRows ? (unsigned)kMaxCluster : 1u, 1, 1};
+  cfg.gridDim = dim3(at[0].val.clusterDim.x), cfg.blockDim = dim3(kThreads), cfg.stream = s, cfg.attrs = at, cfg.numAttrs = 1;
+  LZ_CUDA_TRY(cudaLaunchKernelEx(&cfg, head_kernel<KIND>, *a, order));
+  return LZE_OK;
 }
 
 template <typename T, int KIND>
@@ -366,8 +539,7 @@ int forward_as(const LzLossArgs* a, cudaStream_t s) {
   LzStreamPlan stream;
   if (const int rc = lz_stream_plan(a, &stream)) return rc;
   if (KIND != LZ_LOSS_LOGP || stream.ordered) {
-    head_kernel<KIND><<<1, kThreads, 0, s>>>(*a, stream.ordered);
-    LZ_CUDA_TRY(cudaGetLastError());
+    if (const int rc = launch_head<KIND>(a, stream.ordered, s)) return rc;
   }
   if (!a->rows) return LZE_OK;
   if (stream.clusters) return lz_stream_forward(a, &stream, s);
@@ -386,7 +558,9 @@ int backward_as(const LzLossArgs* a, cudaStream_t s) {
   if (lz_stream_grad_fits(a)) return lz_stream_grad(a, s);
   RowLaunch l;
   if (const int rc = plan_rows(a, &l)) return rc;
-  if (l.team == 32) row_grad_kernel<T, KIND, 32><<<l.grid, kRowThreads, l.smem, s>>>(*a, l.hash);
+  if (KIND != LZ_LOSS_DISTILL && l.team == 8) warp_grad_kernel<T, KIND, 8><<<l.grid, kRowThreads, 0, s>>>(*a, l.batch);
+  else if (KIND != LZ_LOSS_DISTILL && l.team == 16) warp_grad_kernel<T, KIND, 16><<<l.grid, kRowThreads, 0, s>>>(*a, l.batch);
+  else if (l.team == 32) row_grad_kernel<T, KIND, 32><<<l.grid, kRowThreads, l.smem, s>>>(*a, l.hash);
   else row_grad_kernel<T, KIND, kRowThreads><<<l.grid, kRowThreads, l.smem, s>>>(*a, l.hash);
   LZ_CUDA_TRY(cudaGetLastError());
   return LZE_OK;

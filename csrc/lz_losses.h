@@ -41,7 +41,7 @@ struct LzLossArgs {
   unsigned char* clipped;  // [rows] (POLICY)
   // [HEAD + ROW rows], 16-byte aligned: head, then per row its sum (four
   // floats), the slope of the loss in its log-probability (LOGP: that itself, in
-  // 64 bits, since sums of many are taken of it), its loss, and its
+  // 64 bits, since sums of many are taken of it), a CTA's loss, and its
   // place in the order in which rows are taken (int)
   double* work;
   double denom;          // denominator; < 0: the sum of the weights

@@ -24,6 +24,7 @@ namespace {
 constexpr double kLn2 = 0.693147180559945309417;
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr int kMaxDevices = 64;
+constexpr int kMaxCluster = 8;
 constexpr int kSmallList = 128;  // teacher's lists up to here look for equal ids entry by entry, longer ones by a hash table
 
 // 2^x; results below 2^-126 are zero.
@@ -133,6 +134,37 @@ struct Split {
     vecs = (int)((n - lead) / Elem<T>::N);
   }
 };
+
+LZ_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+LZ_DEV uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+LZ_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// `v` of CTA `rank` of this cluster.
+template <typename V>
+LZ_DEV V peer_value(const V* v, uint32_t rank) {
+  static_assert(sizeof(V) == 16, "two words");
+  uint64_t w[2];
+  asm volatile(
+      "{\n\t.reg .b32 p;\n\t"
+      "mapa.shared::cluster.u32 p, %2, %3;\n\t"
+      "ld.shared::cluster.v2.b64 {%0, %1}, [p];\n\t}"
+      : "=l"(w[0]), "=l"(w[1])
+      : "r"(smem_addr(v)), "r"(rank)
+      : "memory");
+  V out;
+  memcpy(&out, w, 16);
+  return out;
+}
 
 // Index of the t-th single element of a row of `n`, or -1.
 LZ_DEV long long single_of(int lead, int vecs, int per_vec, int t, long long n) {
@@ -392,13 +424,37 @@ LZ_DEV RowOut row_out(const LzLossArgs& a, const RowParams& p, const Norm& n, fl
   return o;
 }
 
-// Writes a row's outputs and what the backward pass takes (from which it gets the same
-// bits for upstream 1); returns its loss. `t`: the teacher's list. One warp.
+// Writes (where `store`) a row's outputs and what the backward pass takes, from which it
+// gets the same bits for upstream 1; returns its loss. `kl`: DISTILL's. One thread.
+template <int KIND>
+LZ_DEV double row_write(const LzLossArgs& a, const RowParams& p, const RowOut& o, const RowSum& n, double kl, long long r,
+                        bool store) {
+  double each = kl;
+  if (KIND == LZ_LOSS_POLICY) {
+    const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
+    each = -(double)p.adv * (o.clipped ? (p.adv > 0.f ? hi : lo) : (double)o.ratio);
+    if (a.ref_logp) {
+      const double d = (p.ref_logp2 - o.logp2) * kLn2;
+      kl = expm1(d) - d;
+      each += (double)a.kl_coef * kl;
+    }
+  }
+  if (store) {
+    if (KIND != LZ_LOSS_DISTILL) a.logp[r] = (float)(o.logp2 * kLn2);
+    if (KIND == LZ_LOSS_DISTILL || (KIND == LZ_LOSS_POLICY && a.ref_logp)) a.kl[r] = (float)kl;
+    if (KIND == LZ_LOSS_POLICY) a.clipped[r] = o.clipped;
+    work_sum(a)[r] = make_float4(n.base, n.ref, n.sum, 0.f);
+    work_slope(a)[r] = KIND == LZ_LOSS_LOGP ? o.logp2 * kLn2 : (double)o.slope;
+  }
+  return KIND == LZ_LOSS_LOGP ? 0.0 : p.weight * each;
+}
+
+// The same by one warp. `t`: the teacher's list.
 template <int KIND>
 LZ_DEV double row_outputs(const LzLossArgs& a, const RowParams& p, const RowOut& o, const RowSum& n, const TopView& t,
                           long long r, float c) {
   const int lane = threadIdx.x % 32;
-  double each = 0.0, kl = 0.0;
+  double kl = 0.0;
   if (KIND == LZ_LOSS_DISTILL) {
     kl = p.q_logq - kLn2 * (p.q_z - p.q_sum * o.norm.lse2);
     if (o.norm.base != 0.f) {  // differences of what is beyond 32 bits: entry by entry
@@ -411,25 +467,8 @@ LZ_DEV double row_outputs(const LzLossArgs& a, const RowParams& p, const RowOut&
       for (int s = 16; s; s >>= 1) kl += __shfl_xor_sync(~0u, kl, s);
     }
     if (isnan(p.slope)) kl = NAN;
-    each = kl;
   }
-  if (KIND == LZ_LOSS_POLICY) {
-    const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
-    each = -(double)p.adv * (o.clipped ? (p.adv > 0.f ? hi : lo) : (double)o.ratio);
-    if (a.ref_logp) {
-      const double d = (p.ref_logp2 - o.logp2) * kLn2;
-      kl = expm1(d) - d;
-      each += (double)a.kl_coef * kl;
-    }
-  }
-  if (lane == 0) {
-    if (KIND != LZ_LOSS_DISTILL) a.logp[r] = (float)(o.logp2 * kLn2);
-    if (KIND == LZ_LOSS_DISTILL || (KIND == LZ_LOSS_POLICY && a.ref_logp)) a.kl[r] = (float)kl;
-    if (KIND == LZ_LOSS_POLICY) a.clipped[r] = o.clipped;
-    work_sum(a)[r] = make_float4(n.base, n.ref, n.sum, 0.f);
-    work_slope(a)[r] = KIND == LZ_LOSS_LOGP ? o.logp2 * kLn2 : (double)o.slope;
-  }
-  return KIND == LZ_LOSS_LOGP ? 0.0 : p.weight * each;
+  return row_write<KIND>(a, p, o, n, kl, r, lane == 0);
 }
 
 // A row's slope for the given upstream.
@@ -472,6 +511,20 @@ LZ_DEV void touch_logits(const LzLossArgs& a, const T* x, long long r) {
   }
 }
 
+// A row's scalars (LOGP, POLICY).
+template <typename T, int KIND>
+LZ_DEV void token_params(const LzLossArgs& a, const T* x, long long r, RowParams& out) {
+  const long long y = load_id(a.ids, a.ids64, r);
+  out.token = y < a.vocab ? (int)y : -1;
+  out.xy = y < a.vocab ? Elem<T>::get(x[y]) : 0.f;
+  if (KIND == LZ_LOSS_POLICY) {
+    out.adv = a.advantages[r];
+    out.old_logp2 = (double)a.old_logp[r] * kLog2e;
+    out.ref_logp2 = a.ref_logp ? (double)a.ref_logp[r] * kLog2e : 0.0;
+    out.weight = (a.weights ? (double)a.weights[r] : 1.0) * a.work[0];
+  }
+}
+
 // A row's scalars and, for DISTILL, the teacher's list; `hash` has `hashed` entries, a
 // power of two, where the list is long. One warp.
 template <typename T, int KIND>
@@ -479,17 +532,7 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const T* x, long long r, RowPara
                            float c) {
   const int lane = threadIdx.x % 32;
   if (KIND != LZ_LOSS_DISTILL) {
-    if (lane == 0) {
-      const long long y = load_id(a.ids, a.ids64, r);
-      out.token = y < a.vocab ? (int)y : -1;
-      out.xy = y < a.vocab ? Elem<T>::get(x[y]) : 0.f;
-      if (KIND == LZ_LOSS_POLICY) {
-        out.adv = a.advantages[r];
-        out.old_logp2 = (double)a.old_logp[r] * kLog2e;
-        out.ref_logp2 = a.ref_logp ? (double)a.ref_logp[r] * kLog2e : 0.0;
-        out.weight = (a.weights ? (double)a.weights[r] : 1.0) * a.work[0];
-      }
-    }
+    if (lane == 0) token_params<T, KIND>(a, x, r, out);
     __syncwarp();
     return;
   }

@@ -19,7 +19,6 @@
 namespace {
 
 constexpr int kMaxSlots = 64;
-constexpr int kMaxCluster = 8;
 constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of every wait
 
 // Which row, and this CTA's slice of it.
@@ -44,19 +43,6 @@ struct alignas(128) StreamShared {
   int failed;
 };
 
-LZ_DEV uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-LZ_DEV uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-LZ_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 LZ_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.shared::cta.b64 t, [%0];\n\t}" ::"r"(smem_addr(bar)) : "memory");
 }

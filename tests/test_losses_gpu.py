@@ -752,6 +752,44 @@ def test_many_rows_of_every_kind():
         del case, x
 
 
+@pytest.mark.parametrize("n,v,dtype", [(150001, 8, BF16), (40003, 33, FP16), (20000, 41, FP32), (15000, 1001, BF16),
+                                       (14500, 512, FP32), (14209, 1024, FP16), (5001, 2047, FP16), (9999, 1022, FP32)])
+def test_very_many_short_rows(n, v, dtype):
+    """Rows that a part of a warp has, several at once: ragged batches, rows that do not count in
+    every place, weights, masked entries, rows of huge masks only, and both ways of a gradient."""
+    x, y, old, adv, ref = _policy_case(n, v, dtype, n)
+    big = 6e4 if dtype is FP16 else 1e10
+    x[7::50] = -big
+    x[11::13, v // 2] = -math.inf
+    y = torch.where(y == v // 2, 0, y)
+    y[11::13] = torch.where(y[11::13] == v // 2, 0, y[11::13])
+    lp = oracle.logp64(x, y[:, None], 1.0)[0][:, 0]
+    old, ref = (lp - 0.1 * (old * 7).sin()).float(), (lp + 0.3 * (ref * 5).sin()).float()
+    y[::9] = -1
+    y[n // 3:n // 3 + 70] = -1
+    y[-3:] = -1
+    w = torch.rand(n, device="cuda", generator=_gen(2)) + 0.5
+    w[5::17] = 0
+    _check_policy(x, y, old, adv, ref, w)
+    _check_policy(x, y.int(), old, adv, ref, w, upstream=0.5, denom=77.0)
+    test_token_logprobs_sizes(n, v, dtype)
+
+
+@pytest.mark.parametrize("ids", [torch.int64, torch.int32])
+def test_many_rows_in_order(ids):
+    """More rows than one block sorts, streamed: runs that do not count at either end and in between."""
+    n, v = 3001, 24000
+    x, y, old, adv, ref = _policy_case(n, v, BF16, 4)
+    y[:700], y[1300:1600], y[2990:], y[::11] = -1, -1, -1, -1
+    w = torch.rand(n, device="cuda", generator=_gen(2)) + 0.5
+    w[3::19] = 0
+    _check_policy(x, y.to(ids), old, adv, ref, w)
+    _check_policy(x, y.to(ids), old, adv, ref, None, upstream=0.5)
+    x, idx, t = _distill_case(n, 52000, 20, BF16, 3)
+    _check_distill(x, idx.to(ids), t, w)
+    _check_distill(x, idx.to(ids), t, torch.zeros_like(w))
+
+
 def test_losses_under_autocast_and_checkpoint():
     from torch.utils.checkpoint import checkpoint
 
