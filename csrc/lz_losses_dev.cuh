@@ -593,11 +593,17 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const T* x, long long r, RowPara
   // Does an id stand in the list twice? Then its first entry gets all shares.
   bool twice = false;
   if (a.top <= kSmallList) {
+    // Four ids a load. The last may have words of `z` in it; where one is taken for an id, the list
+    // is looked at again all the same.
+    const int4* four = reinterpret_cast<const int4*>(t.id);
     for (int k = lane; k < a.top; k += 32) {
       const int id = t.id[k];
       int same = 0;
-#pragma unroll 8
-      for (int o = 0; o < a.top; ++o) same += t.id[o] == id;
+#pragma unroll 4
+      for (int o = 0; o < (a.top + 3) / 4; ++o) {
+        const int4 v = four[o];
+        same += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+      }
       twice |= id >= 0 && same > 1;
     }
   } else {
@@ -647,7 +653,8 @@ struct LzStreamPlan {
   int slots;    // of the ring, a chunk each
   int early;    // chunks of the next row taken before this one's gradient
   int ordered;  // rows by work_order; otherwise one row a cluster
-  int hash;     // entries of the hash table of DISTILL, a power of two; 0 where the list is short
+  int hash;     // entries of a hash table of DISTILL, a power of two; 0 where the list is short
+  int views;    // DISTILL: rows whose lists are kept, 2 or 4
   size_t smem;
 };
 int lz_stream_plan(const LzLossArgs* a, LzStreamPlan* plan);

@@ -12,6 +12,7 @@
 // row's outputs, and puts the few entries with t_j != 0 over the dense gradient
 // once that is written. While it does, the W warps take the first chunks of the
 // next row, as many as fit beside this one.
+#include <algorithm>
 #include <atomic>
 
 #include "lz_losses_dev.cuh"
@@ -27,19 +28,22 @@ struct RowHead {
   int lead, vecs, first, count, chunks;
 };
 
-// Both rows' lists (id, z, q, share) and the hash table.
-__host__ __device__ inline int list_bytes(int kind, int top, int hash) {
-  return kind == LZ_LOSS_DISTILL ? (top * 32 + hash * 4 + 127) / 128 * 128 : 0;
+constexpr int kListWarps = 2;
+
+// The lists (id, z, q, share) of `views` rows, and each list warp's hash table.
+__host__ __device__ inline int list_bytes(int kind, int top, int hash, int views) {
+  return kind == LZ_LOSS_DISTILL ? (top * 16 * views + hash * 4 * kListWarps + 127) / 128 * 128 : 0;
 }
 
 struct alignas(128) StreamShared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
-  uint64_t parts[2], peers[2], dense[2], ready[2], used[2];  // of every other row
+  uint64_t parts[2], peers[2], dense[2];  // of every other row
+  uint64_t ready[4], used[4];             // of every row's scalars and list, in turn
   float2 warp_part[2][16];
   float2 peer_part[2][kMaxCluster];
   RowHead heads[4];
   RowGrad grad[2];
-  RowParams params[2];
+  RowParams params[4];
   int failed;
 };
 
@@ -131,10 +135,10 @@ LZ_DEV RowHead slice_of(const T* x, long long row, long long vocab, uint32_t ran
 }
 
 // Warps beside the W that take chunks: one feeds the ring, one has the rows'
-// scalars; DISTILL's lists take one more (about 9000 cycles for 64 entries, of
-// the 15000 that a slice of 150 KB takes; on one warp they were the bound).
+// scalars; DISTILL's lists take two more (about 9000 cycles for 64 entries, of
+// the 15000 that a slice of 150 KB takes), so that short rows need not wait for them.
 template <int KIND>
-constexpr int kHelpers = KIND == LZ_LOSS_DISTILL ? 3 : 2;
+constexpr int kHelpers = KIND == LZ_LOSS_DISTILL ? 2 + kListWarps : 2;
 
 template <typename T, int KIND, bool GRAD, int W>
 __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(const __grid_constant__ LzLossArgs a,
@@ -144,7 +148,8 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
   extern __shared__ __align__(128) char smem[];
   StreamShared& sh = *reinterpret_cast<StreamShared*>(smem);
   char* const lists = smem + sizeof(StreamShared);
-  char* const ring = lists + list_bytes(KIND, a.top, plan.hash);
+  char* const ring = lists + list_bytes(KIND, a.top, plan.hash, plan.views);
+  const uint32_t views = KIND == LZ_LOSS_DISTILL ? plan.views : 2, views_log2 = views == 4 ? 2 : 1;  // rows whose scalars are kept
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
   const long long cluster = blockIdx.x / ranks, clusters = gridDim.x / ranks;
@@ -178,6 +183,8 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       mbar_init(&sh.parts[k], W);
       mbar_init(&sh.peers[k], 1);
       mbar_init(&sh.dense[k], 1);
+    }
+    for (int k = 0; k < 4; ++k) {
       mbar_init(&sh.ready[k], 1);
       mbar_init(&sh.used[k], 1);
     }
@@ -309,16 +316,17 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         if (single >= 0) out[single] = Elem<T>::put(0.f);
       }
     }
-  } else if (KIND == LZ_LOSS_DISTILL && warp == W + 2) {  // ---- the teacher's lists, a row ahead
-    int* const hash = reinterpret_cast<int*>(lists) + 8 * a.top;
+  } else if (KIND == LZ_LOSS_DISTILL && warp >= W + 2) {  // ---- the teacher's lists, by one warp or in turns
+    const uint32_t mine = warp - (W + 2);
+    int* const hash = reinterpret_cast<int*>(lists) + 4 * views * a.top + mine * plan.hash;
     long long r, to_come;
-    for (uint32_t turn = 0; row_at(cluster + (long long)turn * clusters, &r); ++turn) {
-      const int k = turn & 1;
-      if (row_at(cluster + (long long)(turn + 2) * clusters, &to_come)) touch_list(a, to_come);
-      if (turn >= 2) ring_wait<false>(&sh.used[k], ((turn - 2) >> 1) & 1, failed);
+    for (uint32_t turn = mine; mine < views / 2 && row_at(cluster + (long long)turn * clusters, &r); turn += views / 2) {
+      const int k = turn & (views - 1);
+      if (row_at(cluster + (long long)(turn + views) * clusters, &to_come)) touch_list(a, to_come);
+      if (turn >= views) ring_wait<false>(&sh.used[k], ((turn >> views_log2) - 1) & 1, failed);
       prepare_params<T, KIND>(a, row_of<T>(a, r), r, sh.params[k], view(k), hash, plan.hash, c);
       if (lane == 0) mbar_arrive(&sh.ready[k]);
-      if (row_at(cluster + (long long)(turn + 1) * clusters, &to_come))
+      if (row_at(cluster + (long long)(turn + views / 2) * clusters, &to_come))
         touch_logits(a, row_of<T>(a, to_come), to_come);
     }
     __syncwarp();
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     for (;; ++turn) {
       const RowHead h = sh.heads[turn & 3];
       if (h.row < 0) break;
-      const int k = turn & 1;
+      const int k = turn & 1, at = turn & (views - 1), last = (turn - 1) & (views - 1);
       const RowHead later = head_at(cluster + (long long)(turn + 2) * clusters);
       ring_wait<false>(&sh.parts[k], (turn >> 1) & 1, failed);
       float2 v = lane < W ? sh.warp_part[k][lane] : make_float2(-INFINITY, 0.f);
@@ -369,8 +377,8 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       }
       RowSum n = {0.f, v.x, v.y};
       if (!exact_ref(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
-      if (KIND == LZ_LOSS_DISTILL) ring_wait<false>(&sh.ready[k], (turn >> 1) & 1, failed);
-      const RowParams& p = sh.params[k];
+      if (KIND == LZ_LOSS_DISTILL) ring_wait<false>(&sh.ready[at], (turn >> views_log2) & 1, failed);
+      const RowParams& p = sh.params[at];
       const RowOut o = row_out<KIND>(a, p, n.norm(), c);
       const RowGrad g(o.slope, a.inv_temperature, n);
       if (lane == 0) {
@@ -378,17 +386,17 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         sh.heads[(turn + 2) & 3] = later;
         mbar_arrive(&sh.dense[k]);
       }
-      sparse(k ^ 1);
+      sparse(last);
       __syncwarp();
-      if (KIND == LZ_LOSS_DISTILL && turn && lane == 0) mbar_arrive(&sh.used[k ^ 1]);  // by the row before
-      if (rank == 0) loss += row_outputs<KIND>(a, p, o, n, view(k), h.row, c);
+      if (KIND == LZ_LOSS_DISTILL && turn && lane == 0) mbar_arrive(&sh.used[last]);  // by the row before
+      if (rank == 0) loss += row_outputs<KIND>(a, p, o, n, view(at), h.row, c);
       before = h, before_grad = g, before_xy = p.xy, before_token = p.token;
       __syncwarp();
       prepare(sh.heads[(turn + 1) & 3], k ^ 1);
     }
     if (GRAD) {
       ring_wait<false>(&sh.parts[turn & 1], (turn >> 1) & 1, failed);
-      sparse((turn & 1) ^ 1);
+      sparse((turn - 1) & (views - 1));
     }
     if (rank == 0) {
       long long r;
@@ -571,17 +579,17 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
 
 // Whether rows are streamed: not small, and each row and its gradient at the same
 // offset from a 16-byte border. A row costs a cluster some 5000 cycles besides its
-// bytes (DISTILL's list 10000), which the many teams of row_kernel hide better
+// bytes, which the many teams of row_kernel hide better
 // while rows are short; it reads a row that outgrows the caches a second time. In
 // us, bf16, streamed against teams: 8192 rows of 64 KB, sums only 130 / 96, 4096 of
 // 300 KB 194 / 204; 8192 with the policy's gradient 32 KB 171 / 140, 64 KB 208 / 259;
-// with DISTILL's of 64 entries 64 KB 371 / 286, 100 KB 394 / 464; the gradient
-// alone, 1024 rows of 64 KB 25 / 21, 8192 rows of 100 KB 256 / 266. Few rows are
+// with DISTILL's of 64 entries 48 KB 201 / 218, 64 KB 236 / 287, but 1024 rows of
+// 64 KB 48 / 42, of 100 KB 63 / 70; the gradient alone, 1024 rows of 64 KB 25 / 21, 8192 rows of 100 KB 256 / 266. Few rows are
 // streamed whatever their length, since a cluster splits them.
 template <typename T>
 bool streams(const LzLossArgs* a, bool forward, bool grad) {
   const long long size = sizeof(T), row = a->vocab * size;
-  const long long from = a->rows <= 64 && forward ? 16 : !forward ? 64 : !grad ? 128 : a->kind == LZ_LOSS_DISTILL ? 96 : 40;
+  const long long from = a->rows <= 64 && forward ? 16 : !forward ? 64 : !grad ? 128 : a->kind != LZ_LOSS_DISTILL || a->rows >= 4096 ? 40 : 80;
   if (row < from * 1024 || a->rows > INT32_MAX) return false;
   if (!grad) return true;
   return ((uintptr_t)a->logits ^ (uintptr_t)a->grad) % 16 == 0 &&
@@ -600,8 +608,9 @@ int plan_as(const LzLossArgs* a, LzStreamPlan* l) {
   int hash = 0;
   if (KIND == LZ_LOSS_DISTILL && a->top > kSmallList)
     for (hash = 32; hash < 2 * a->top;) hash *= 2;
-  const int fixed = (int)sizeof(StreamShared) + list_bytes(KIND, a->top, hash);
-  const int slots = (kSharedMax - fixed) / kChunk < kMaxSlots ? (kSharedMax - fixed) / kChunk : kMaxSlots;
+  const int two = (int)sizeof(StreamShared) + list_bytes(KIND, a->top, hash, 2);
+  const int four = (int)sizeof(StreamShared) + list_bytes(KIND, a->top, hash, 4);
+  const int slots = std::min((kSharedMax - two) / kChunk, kMaxSlots);
   auto kernel = stream_kernel<T, KIND, GRAD, kStreamWarps>;
   static std::atomic<bool> known[kMaxDevices];
   static std::atomic<int> resident[kMaxDevices][kMaxCluster];
@@ -622,6 +631,7 @@ int plan_as(const LzLossArgs* a, LzStreamPlan* l) {
   }
   double best = 0.0;
   int chunks = 0;
+  long long part = 0;
   for (int k = 0; k < kMaxCluster; ++k) {
     const int ranks = k + 1, g = resident[a->device][k].load(std::memory_order_relaxed);
     const long long slice = (row + ranks - 1) / ranks;
@@ -631,9 +641,14 @@ int plan_as(const LzLossArgs* a, LzStreamPlan* l) {
     best = cost;
     l->ranks = ranks;
     l->clusters = (int)(a->rows < g ? a->rows : g);
-    chunks = (int)((slice + 16 + kChunk - 1) / kChunk);
+    chunks = (int)((slice + 16 + kChunk - 1) / kChunk), part = slice;
   }
   l->slots = slots, l->early = slots - chunks, l->ordered = a->rows > l->clusters, l->hash = hash;
+  // Lists of four rows where a list takes longer than a row (8192 rows of 64 KB 371 us, 236 with
+  // four) and the ring loses no slot. With two, a list's logits are read when its row is on the
+  // way to L2 (4096 rows of 300 KB 425 us, with four 438).
+  l->views = part <= 128 * 1024 && (kSharedMax - four) / kChunk >= slots ? 4 : 2;
+  const int fixed = l->views == 4 ? four : two;
   l->smem = fixed + (size_t)slots * kChunk;
   return LZE_OK;
 }
