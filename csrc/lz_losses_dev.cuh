@@ -471,13 +471,13 @@ LZ_DEV double row_outputs(const LzLossArgs& a, const RowParams& p, const RowOut&
   return row_write<KIND>(a, p, o, n, kl, r, lane == 0);
 }
 
-// A row's slope for the given upstream.
+// A row's slope for the given upstream; zero where the row does not count or has no upstream of its own,
+// whatever its token. One beyond the vocabulary is NaN otherwise (POLICY's saved slope is that already).
 template <int KIND>
 LZ_DEV double row_slope_for(const LzLossArgs& a, long long r, long long y, float up) {
-  if (y >= a.vocab) return NAN;
-  if (KIND == LZ_LOSS_LOGP) return y < 0 ? 0.0 : (double)up * (double)a.row_upstream[r];
-  const double slope = work_slope(a)[r];
-  return slope == 0.0 ? 0.0 : (double)up * slope;
+  const double slope = KIND != LZ_LOSS_LOGP ? work_slope(a)[r] : y < 0 ? 0.0 : (double)a.row_upstream[r];
+  if (slope == 0.0) return 0.0;
+  return KIND == LZ_LOSS_LOGP && y >= a.vocab ? (double)NAN : (double)up * slope;
 }
 
 // Outputs of a row that does not count.

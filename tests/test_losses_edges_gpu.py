@@ -1,0 +1,60 @@
+"""Vocabulary losses on the GPU at the edges of what their arguments may hold:
+ids beyond the vocabulary in rows that do not count, teachers without a finite
+entry, scores far apart, saved tensors that come back in another layout, and
+backward passes captured apart from their forward pass."""
+import math
+
+import pytest
+import torch
+
+import results_b200 as lz
+from tests import _losses as oracle
+from tests.test_losses_gpu import BF16, FP16, FP32, _check_distill, _check_policy, _distill_case, _gen, _logits, _policy_case, _tokens
+
+pytestmark = pytest.mark.gpu
+
+# rows that a part of a warp, a warp, a block and a cluster has, in the backward pass too
+KERNELS = [(20000, 64, BF16), (6, 1000, BF16), (7, 30011, FP16), (6, 40000, BF16)]
+
+
+@pytest.mark.parametrize("n,v,dtype", KERNELS)
+def test_bad_tokens_of_rows_without_weight(n, v, dtype):
+    """A padding id beyond the vocabulary in a row of weight zero: gradient zero, whatever the upstream."""
+    x, y, old, adv, ref = _policy_case(n, v, dtype, 1)
+    w = torch.ones(n, device="cuda")
+    w[1] = w[n - 1] = 0
+    bad = y.clone()
+    bad[1], bad[n - 1] = v, 2**40
+    x.requires_grad_(True)
+    for up in (1.0, 2.0):
+        up = torch.tensor(up, device="cuda")
+        want, = torch.autograd.grad(lz.policy_loss(x, y, old, adv, ref_logp=ref, weights=w, kl_coef=0.1).loss, x, up)
+        loss = lz.policy_loss(x, bad, old, adv, ref_logp=ref, weights=w, kl_coef=0.1).loss
+        assert torch.isfinite(loss) and torch.isfinite(want).all()
+        for _ in range(2):  # a second pass computes it anew
+            grad, = torch.autograd.grad(loss, x, up, retain_graph=True)
+            assert torch.equal(grad, want)
+    # and one that counts is NaN in every way
+    bad[0] = v
+    loss = lz.policy_loss(x, bad, old, adv, weights=w).loss
+    for up in (1.0, 2.0):
+        grad, = torch.autograd.grad(loss, x, torch.tensor(up, device="cuda"), retain_graph=True)
+        assert loss.isnan() and grad[0].isnan().all() and torch.isfinite(grad[1:]).all()
+
+
+@pytest.mark.parametrize("n,v,dtype", KERNELS)
+def test_bad_tokens_outside_of_the_sequences(n, v, dtype):
+    """The tail of a packed buffer that nobody wrote, and log-probabilities that a user's loss leaves out."""
+    x, y = _logits(n, v, dtype, 1).requires_grad_(True), _tokens(n, v, 2)
+    cu = torch.tensor([1, 2, 3, 4, 5], device="cuda")
+    bad = y.clone()
+    bad[0], bad[5], bad[n - 1] = v, v + 5, 2**40
+    for up in (1.0, 0.5):
+        up = torch.tensor(up, device="cuda")
+        want, = torch.autograd.grad(lz.preference_loss(x, y, cu_seqlens=cu).loss, x, up)
+        loss = lz.preference_loss(x, bad, cu_seqlens=cu).loss
+        grad, = torch.autograd.grad(loss, x, up)
+        assert torch.isfinite(loss) and torch.equal(grad, want) and torch.all(grad[5:] == 0)
+    logp = lz.token_logprobs(x, bad)
+    grad, = torch.autograd.grad(torch.where(logp.isnan(), 0.0, logp).sum(), x)
+    assert torch.all(grad[[0, 5, n - 1]] == 0) and torch.isfinite(grad).all() and logp.isnan().sum() == len({0, 5, n - 1})
