@@ -315,12 +315,24 @@ class _PairsCall(_Call):
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------
 
 
+def _cpu_nan_rows(x, bad):
+    """x [rows], NaN where `bad`, and its gradient there as well, unless the row has no upstream."""
+    if x.requires_grad and bool(bad.any()):
+        x.register_hook(lambda g: torch.where(bad & (g != 0), math.nan, g))
+    return x + torch.where(bad, math.nan, 0.0)
+
+
 def _cpu_logp(logits, ids, counted, temperature):
     """Log-probabilities of ids [rows, k] in 64 bits; rows that do not count are not looked at."""
     v = logits.shape[-1]
     z = torch.where(counted[:, None], logits.reshape(-1, v).double(), 0.0) / temperature
-    logp = torch.log_softmax(z, -1).gather(1, ids.clamp(0, v - 1).long())
-    return torch.where((ids >= v) & counted[:, None], math.nan, logp)
+    return torch.log_softmax(z, -1).gather(1, ids.clamp(0, v - 1).long())
+
+
+def _cpu_token_logp(logits, y, counted, temperature):
+    """Log-probabilities of tokens [rows], zero where a row does not count."""
+    logp = _cpu_nan_rows(_cpu_logp(logits, y[:, None], counted, temperature)[:, 0], counted & (y >= logits.shape[-1]))
+    return torch.where(counted, logp, 0.0)
 
 
 def _cpu_scale(weights, counted, denom):
@@ -331,8 +343,7 @@ def _cpu_scale(weights, counted, denom):
 
 def _cpu_token_logprobs(logits, tokens, temperature):
     y = tokens.reshape(-1)
-    logp = _cpu_logp(logits, y[:, None], y >= 0, temperature)[:, 0]
-    return torch.where(y >= 0, logp, 0.0).float().view(tokens.shape)
+    return _cpu_token_logp(logits, y, y >= 0, temperature).float().view(tokens.shape)
 
 
 def _cpu_policy_loss(logits, tokens, rows, p):
@@ -340,7 +351,7 @@ def _cpu_policy_loss(logits, tokens, rows, p):
     y = tokens.reshape(-1)
     scale = _cpu_scale(weights, y >= 0, p["denom"])
     counted = (y >= 0) & (weights != 0) if weights is not None else y >= 0
-    logp = torch.where(counted, _cpu_logp(logits, y[:, None], counted, p["temperature"])[:, 0], 0.0)
+    logp = _cpu_token_logp(logits, y, counted, p["temperature"])
     ratio = torch.where(counted, logp - old, 0.0).exp()
     low, high = 1.0 - p["clip_low"], 1.0 + p["clip_high"]
     clipped = (((adv > 0) & (ratio > high)) | ((adv < 0) & (ratio < low))) & counted
@@ -364,9 +375,10 @@ def _cpu_distill_loss(logits, ids, teacher, weights, p):
     some = t.amax(1) != -math.inf
     logq = torch.log_softmax(torch.where(some[:, None], t, 0.0), 1)
     q = torch.where(there & some[:, None], logq.exp(), 0.0)
+    bad = (q.isnan() | (ids >= logits.shape[-1])).any(1) & counted
+    q, logq = torch.where(bad[:, None], 1.0, q), torch.where(bad[:, None], 0.0, logq)
     logp = _cpu_logp(logits, ids, counted & some, p["temperature"])
-    kl = torch.where(q > 0, q * (logq - logp), 0.0)
-    kl = torch.where(q.isnan() | (ids >= logits.shape[-1]), math.nan, kl).sum(1)
+    kl = _cpu_nan_rows(torch.where(q > 0, q * (logq - logp), 0.0).sum(1), bad)
     kl = torch.where(counted, kl, 0.0)
     loss = (kl * _cpu_scale(weights, torch.ones_like(counted), p["denom"])).sum().float()
     return loss, kl.detach().float().view(logits.shape[:-1])
@@ -374,7 +386,7 @@ def _cpu_distill_loss(logits, ids, teacher, weights, p):
 
 def _cpu_preference_loss(logits, tokens, ref, offsets, p):
     y, pairs = tokens.reshape(-1), p["pairs"]
-    logp = torch.where(y >= 0, _cpu_logp(logits, y[:, None], y >= 0, p["temperature"])[:, 0], 0.0)
+    logp = _cpu_token_logp(logits, y, y >= 0, p["temperature"])
     ends = [s * p["length"] for s in range(2 * pairs + 1)] if offsets is None else offsets.tolist()
     sums = []
     for a, b in zip(ends, ends[1:]):

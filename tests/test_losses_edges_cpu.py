@@ -1,0 +1,58 @@
+"""Vocabulary losses on CPU tensors at the edges of what their arguments may hold."""
+import math
+
+import pytest
+import torch
+
+import results_b200 as lz
+
+
+def _g(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _inputs(n, v, seed=1):
+    x = torch.randn(n, v, generator=_g(seed)).requires_grad_(True)
+    return x, torch.randint(0, v, (n,), generator=_g(seed + 1)), torch.zeros(n)
+
+
+def test_gradients_of_ids_beyond_the_vocabulary():
+    """NaN in the rows that count, zero in those that do not."""
+    x, y, z = _inputs(6, 8)
+    y[1], y[2] = 8, 2**40
+    w = torch.tensor([1.0, 1, 0, 1, 1, 1])
+    for up in (1.0, 2.0):
+        out = lz.token_logprobs(x, y)
+        grad, = torch.autograd.grad((out * up).sum(), x)
+        assert grad[1:3].isnan().all() and torch.isfinite(grad[[0, 3, 4, 5]]).all()
+        out = lz.policy_loss(x, y, z, z + 1, weights=w)
+        grad, = torch.autograd.grad(out.loss * up, x)
+        assert out.loss.isnan() and grad[1].isnan().all() and torch.isfinite(grad[[0, 3, 4, 5]]).all() and torch.all(grad[2] == 0)
+        out = lz.preference_loss(x, y, cu_seqlens=torch.tensor([3, 4, 6]))
+        grad, = torch.autograd.grad(out.loss * up, x)
+        assert torch.isfinite(out.loss) and torch.isfinite(grad).all() and torch.all(grad[:3] == 0)
+        ids = torch.stack([torch.zeros_like(y), y], 1)
+        t = torch.zeros(6, 2)
+        t[1, 1] = -math.inf  # an entry of no weight is looked at all the same
+        out = lz.distill_loss(x, ids, t, weights=w)
+        grad, = torch.autograd.grad(out.loss * up, x)
+        assert out.kl.isnan().tolist() == [False, True, False, False, False, False]
+        assert grad[1].isnan().all() and torch.isfinite(grad[[0, 3, 4, 5]]).all() and torch.all(grad[2] == 0)
+    logp = lz.token_logprobs(x, y)
+    grad, = torch.autograd.grad(torch.where(logp.isnan(), 0.0, logp).sum(), x)
+    assert torch.all(grad[1:3] == 0) and torch.isfinite(grad).all()
+
+
+def test_gradient_of_a_teacher_without_a_number():
+    x, y, _ = _inputs(5, 8)
+    ids = torch.stack([y, (y + 1) % 8, (y + 2) % 8], 1)
+    for value in (math.nan, math.inf):
+        t = torch.randn(5, 3, generator=_g(3))
+        t[1, 0] = value
+        t[2] = value
+        t[3, 1], ids[3, 1] = value, -1  # padding
+        t[4] = value
+        out = lz.distill_loss(x, ids, t, weights=torch.tensor([1.0, 1, 1, 1, 0]))
+        grad, = torch.autograd.grad(out.loss, x)
+        assert out.kl.isnan().tolist() == [False, True, True, False, False]
+        assert grad[1:3].isnan().all() and torch.isfinite(grad[[0, 3, 4]]).all() and torch.all(grad[4] == 0)
