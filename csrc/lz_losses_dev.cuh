@@ -466,6 +466,7 @@ LZ_DEV double row_outputs(const LzLossArgs& a, const RowParams& p, const RowOut&
 #pragma unroll
       for (int s = 16; s; s >>= 1) kl += __shfl_xor_sync(~0u, kl, s);
     }
+    if (p.q_sum == 0.0) kl = 0.0;  // an empty list shields its row, whatever the logits are
     if (isnan(p.slope)) kl = NAN;
   }
   return row_write<KIND>(a, p, o, n, kl, r, lane == 0);

@@ -56,3 +56,14 @@ def test_gradient_of_a_teacher_without_a_number():
         grad, = torch.autograd.grad(out.loss, x)
         assert out.kl.isnan().tolist() == [False, True, True, False, False]
         assert grad[1:3].isnan().all() and torch.isfinite(grad[[0, 3, 4]]).all() and torch.all(grad[4] == 0)
+
+
+def test_an_empty_list_shields_its_row():
+    x, y, _ = _inputs(5, 8)
+    with torch.no_grad():
+        x[1, 3], x[2, 4], x[3] = math.nan, math.inf, -math.inf
+    ids, t = torch.stack([y, (y + 1) % 8], 1), torch.randn(5, 2, generator=_g(3))
+    ids[1:3], t[3] = -1, -math.inf
+    out = lz.distill_loss(x, ids, t)
+    grad, = torch.autograd.grad(out.loss, x)
+    assert torch.isfinite(out.loss) and torch.all(out.kl[1:4] == 0) and torch.all(grad[1:4] == 0) and torch.isfinite(grad).all()

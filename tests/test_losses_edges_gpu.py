@@ -58,3 +58,25 @@ def test_bad_tokens_outside_of_the_sequences(n, v, dtype):
     logp = lz.token_logprobs(x, bad)
     grad, = torch.autograd.grad(torch.where(logp.isnan(), 0.0, logp).sum(), x)
     assert torch.all(grad[[0, 5, n - 1]] == 0) and torch.isfinite(grad).all() and logp.isnan().sum() == len({0, 5, n - 1})
+
+
+@pytest.mark.parametrize("v", [40, 1003, 40000, 151552])
+@pytest.mark.parametrize("k", [1, 5, 300])
+@pytest.mark.parametrize("upstream", [1.0, 2.0])
+def test_an_empty_list_shields_its_row(v, k, upstream):
+    """A padding row is marked by its list alone; its logits are whatever was there."""
+    x, ids, t = _distill_case(6, v, min(k, v), BF16, 3)
+    x[1, v // 2], x[2, v // 3], x[3] = math.nan, math.inf, -math.inf
+    ids[1:3] = -1
+    t[3] = -math.inf
+    leaf = x.clone().requires_grad_(True)
+    out = lz.distill_loss(leaf, ids, t)
+    grad, = torch.autograd.grad(out.loss, leaf, torch.tensor(upstream, device="cuda"))
+    with torch.no_grad():
+        assert torch.equal(lz.distill_loss(x, ids, t).kl[1:4], out.kl[1:4])
+    assert torch.all(out.kl[1:4] == 0) and torch.all(grad[1:4] == 0)
+    x[1:4] = 0  # the others are the formula's
+    w = torch.tensor([1.0, 0, 0, 0, 1, 1], device="cuda")
+    want = lz.distill_loss(x.requires_grad_(True), ids, t, weights=w, denom=6.0)
+    assert torch.equal(want.loss, out.loss)
+    assert torch.equal(grad, torch.autograd.grad(want.loss, x, torch.tensor(upstream, device="cuda"))[0])
