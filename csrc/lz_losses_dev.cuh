@@ -556,7 +556,7 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const T* x, long long r, RowPara
       const int k = first + 32 * u + lane;
       if (k >= a.top) break;
       if (id[u] < 0) v[u] = -INFINITY;
-      bad |= id[u] >= a.vocab;
+      bad |= id[u] >= a.vocab || (id[u] >= 0 && !(v[u] < INFINITY));  // NaN: the maximum would pass over it
       t.id[k] = id[u] >= 0 && id[u] < a.vocab ? (int)id[u] : -1;
       t.z[k] = Elem<T>::get(z[u]);
       t.q[k] = v[u];
@@ -572,7 +572,7 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const T* x, long long r, RowPara
   for (int k = lane; k < a.top; k += 32) {
     const float v = t.q[k] - m, e = m == -INFINITY ? 0.f : expf(v);
     t.q[k] = e;
-    if (e != 0.f) {  // NaN counts
+    if (e != 0.f) {
       s += e;
       e_v += (double)e * (double)v;
       e_z += (double)e * ((double)t.z[k] * (double)c);

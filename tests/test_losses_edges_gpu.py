@@ -80,3 +80,28 @@ def test_an_empty_list_shields_its_row(v, k, upstream):
     want = lz.distill_loss(x.requires_grad_(True), ids, t, weights=w, denom=6.0)
     assert torch.equal(want.loss, out.loss)
     assert torch.equal(grad, torch.autograd.grad(want.loss, x, torch.tensor(upstream, device="cuda"))[0])
+
+
+@pytest.mark.parametrize("v", [40, 1003, 40000, 151552])
+@pytest.mark.parametrize("k", [1, 5, 300])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_teacher_without_a_number_shows(v, k, value):
+    """One NaN or +inf among a row's entries, nothing else, and nothing else but padding or -inf; not in an
+    entry that is padding, and not in a row without weight."""
+    x, ids, t = _distill_case(7, v, min(k, v), FP32, 3)
+    t[1, 0] = value
+    t[2] = value
+    t[3], ids[3, 1:] = value, -1
+    t[4], t[4, 0] = -math.inf, value
+    t[5, 0], ids[5, 0] = value, -1
+    t[6] = value
+    w = torch.ones(7, device="cuda")
+    w[6] = 0
+    leaf = x.requires_grad_(True)
+    for upstream in (1.0, 2.0):
+        out = lz.distill_loss(leaf, ids, t, weights=w)
+        grad, = torch.autograd.grad(out.loss, leaf, torch.tensor(upstream, device="cuda"))
+        assert out.loss.isnan() and out.kl.isnan().tolist() == [False, True, True, True, True, False, False]
+        assert grad[1:5].isnan().all() and torch.isfinite(grad[[0, 5, 6]]).all()
+    with torch.no_grad():
+        assert torch.equal(lz.distill_loss(x, ids, t, weights=w).kl.isnan(), out.kl.isnan())
