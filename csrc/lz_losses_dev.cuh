@@ -396,9 +396,7 @@ struct TopView {
   float *z, *q, *share;  // share < 0: another entry of the same id has it
 };
 
-LZ_DEV float top_value(const LzLossArgs& a, long long r, int k) {
-  return load_any(a.teacher, a.teacher_dtype, r * a.top + k) * a.inv_temperature;
-}
+LZ_DEV float top_value(const LzLossArgs& a, long long r, int k) { return load_any(a.teacher, a.teacher_dtype, r * a.top + k); }
 
 // What a row's scalars give; logp2: the token's log-probability in base 2.
 struct RowOut {
@@ -566,11 +564,11 @@ LZ_DEV void prepare_params(const LzLossArgs& a, const T* x, long long r, RowPara
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   bad = __any_sync(~0u, bad);
-  // Sums over e = exp(v - m); q = e / s.
+  // Sums over e = exp((v - m) / T); q = e / s. The difference comes first: a type's lowest value over T may be -inf.
   float s = 0.f;
   double e_v = 0.0, e_z = 0.0;
   for (int k = lane; k < a.top; k += 32) {
-    const float v = t.q[k] - m, e = m == -INFINITY ? 0.f : expf(v);
+    const float v = (t.q[k] - m) * a.inv_temperature, e = m == -INFINITY ? 0.f : expf(v);
     t.q[k] = e;
     if (e != 0.f) {
       s += e;

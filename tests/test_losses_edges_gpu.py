@@ -105,3 +105,18 @@ def test_a_teacher_without_a_number_shows(v, k, value):
         assert grad[1:5].isnan().all() and torch.isfinite(grad[[0, 5, 6]]).all()
     with torch.no_grad():
         assert torch.equal(lz.distill_loss(x, ids, t, weights=w).kl.isnan(), out.kl.isnan())
+
+
+@pytest.mark.parametrize("v", [40, 40000])
+@pytest.mark.parametrize("temperature", [0.25, 1.0, 3.0])
+def test_a_teacher_at_its_types_ends(v, temperature):
+    """Lists of the lowest value alone (all entries equal) or beside others, and of the largest."""
+    x, ids, _ = _distill_case(4, v, 9, FP32, 3)
+    for dtype in (FP32, BF16, FP16):
+        low = torch.finfo(dtype).min
+        t = torch.randn(4, 9, device="cuda", generator=_gen(1)).to(dtype)
+        t[0] = low
+        t[1, 3:] = low
+        t[2] = -low
+        t[3, 4], t[3, 5:] = -low, low
+        _check_distill(x, ids, t, temperature=temperature)
