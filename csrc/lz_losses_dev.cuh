@@ -13,6 +13,7 @@
 // the loss) in 64 bits, since a log-probability enters the KL term and the
 // ratio as a difference and costs nothing per element.
 #pragma once
+#include <cfloat>
 #include <type_traits>
 
 #include "lz_common.cuh"
@@ -416,7 +417,7 @@ LZ_DEV RowOut row_out(const LzLossArgs& a, const RowParams& p, const Norm& n, fl
     o.ratio = exp2f((float)(o.logp2 - p.old_logp2));
     o.clipped = (p.adv > 0.f && o.ratio > 1.f + a.clip_high) || (p.adv < 0.f && o.ratio < 1.f - a.clip_low);
     float slope = o.clipped ? 0.f : -p.adv * o.ratio;
-    if (a.ref_logp) slope -= a.kl_coef * expm1f((float)((p.ref_logp2 - o.logp2) * kLn2));
+    if (a.kl_coef != 0.f) slope -= a.kl_coef * expm1f((float)((p.ref_logp2 - o.logp2) * kLn2));
     o.slope = (float)(p.weight * (double)slope);
   }
   return o;
@@ -433,8 +434,8 @@ LZ_DEV double row_write(const LzLossArgs& a, const RowParams& p, const RowOut& o
     each = -(double)p.adv * (o.clipped ? (p.adv > 0.f ? hi : lo) : (double)o.ratio);
     if (a.ref_logp) {
       const double d = (p.ref_logp2 - o.logp2) * kLn2;
-      kl = expm1(d) - d;
-      each += (double)a.kl_coef * kl;
+      kl = expm1(d) - fmin(d, DBL_MAX);  // +inf where the token has probability zero
+      if (a.kl_coef != 0.f) each += (double)a.kl_coef * kl;  // 0: watched alone, it may be infinite
     }
   }
   if (store) {

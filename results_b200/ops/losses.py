@@ -359,8 +359,9 @@ def _cpu_policy_loss(logits, tokens, rows, p):
     kl = None
     if ref is not None:
         d = torch.where(counted, ref - logp, 0.0)
-        kl = d.expm1() - d
-        each = each + p["kl_coef"] * kl
+        kl = d.expm1() - d.clamp(max=torch.finfo(torch.float64).max)  # +inf where the token has probability zero
+        if p["kl_coef"]:  # 0: watched alone, it may be infinite
+            each = each + p["kl_coef"] * kl
         kl = kl.detach().float().view(tokens.shape)
     loss = torch.where(counted, each * scale, 0.0).sum().float()
     return loss, logp.detach().float().view(tokens.shape), kl, clipped.view(tokens.shape)
@@ -433,7 +434,7 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
         loss  = sum(weights each) / denom
 
     ``old_logp``, ``advantages``, ``ref_logp`` and ``weights`` (a mask or
-    factors) have the tokens' shape. ``denom`` is a number or a one-element
+    factors) have the tokens' shape. With ``kl_coef`` 0 the KL is an output alone. ``denom`` is a number or a one-element
     tensor on the device (the token count over all micro batches or ranks);
     without it, the sum of the weights of the rows that count. Where that is
     not positive, loss and gradient are zero."""

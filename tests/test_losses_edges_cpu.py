@@ -67,3 +67,14 @@ def test_an_empty_list_shields_its_row():
     out = lz.distill_loss(x, ids, t)
     grad, = torch.autograd.grad(out.loss, x)
     assert torch.isfinite(out.loss) and torch.all(out.kl[1:4] == 0) and torch.all(grad[1:4] == 0) and torch.isfinite(grad).all()
+
+
+def test_a_watched_kl_changes_nothing():
+    x, y, z = _inputs(4, 8)
+    with torch.no_grad():
+        x[1, y[1]], x[2, y[2]] = -1000, -math.inf
+    out = lz.policy_loss(x, y, z - 2, z + 1, ref_logp=z - 1)
+    plain = lz.policy_loss(x, y, z - 2, z + 1)
+    assert torch.equal(out.loss, plain.loss) and torch.isfinite(out.loss) and torch.all(out.kl[1:3] == math.inf)
+    a, b = (torch.autograd.grad(o.loss, x)[0] for o in (out, plain))
+    assert torch.isfinite(a).all() and torch.equal(a, b)

@@ -120,3 +120,22 @@ def test_a_teacher_at_its_types_ends(v, temperature):
         t[2] = -low
         t[3, 4], t[3, 5:] = -low, low
         _check_distill(x, ids, t, temperature=temperature)
+
+
+@pytest.mark.parametrize("v", [40, 1003, 40000])
+@pytest.mark.parametrize("low", [-100.0, -1000.0])
+def test_a_watched_kl_changes_nothing(v, low):
+    """kl_coef 0: the KL is an output alone, however far a token is below its reference."""
+    x = _logits(4, v, FP32, 1)
+    y = _tokens(4, v, 2)
+    x[1, y[1]] = low
+    x[2, y[2]] = -math.inf
+    lp = oracle.logp64(x, y[:, None], 1.0)[0][:, 0]
+    old, adv = torch.where(lp.isfinite(), lp, 0.0).float() + 0.1, torch.ones(4, device="cuda")
+    x.requires_grad_(True)
+    out = lz.policy_loss(x, y, old, adv, ref_logp=torch.full((4,), -1.0, device="cuda"))
+    plain = lz.policy_loss(x, y, old, adv)
+    assert torch.equal(out.loss, plain.loss) and torch.isfinite(out.loss) and out.kl[1] > 1e38 and out.kl[2] == math.inf
+    for up in (1.0, 2.0):
+        a, b = (torch.autograd.grad(o.loss, x, torch.tensor(up, device="cuda"), retain_graph=True)[0] for o in (out, plain))
+        assert torch.isfinite(a).all() and torch.equal(a, b)
