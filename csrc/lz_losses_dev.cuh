@@ -403,22 +403,37 @@ LZ_DEV float top_value(const LzLossArgs& a, long long r, int k) { return load_an
 struct RowOut {
   double logp2;
   Norm norm;
-  float ratio, slope;
+  double ratio;
+  float slope;
   bool clipped;
 };
+
+// 2^x in the range of 64 bits, to the precision of 32: ratios beyond fp32 may be brought back by the
+// advantage, the weight or the denominator, and the integer part of x takes no bits from the rest.
+LZ_DEV double exp2_wide(double x) {
+  if (!(fabs(x) < 1500.0)) return x < 0.0 ? 0.0 : x > 0.0 ? (double)INFINITY : x;  // x: NaN
+  const double whole = rint(x);
+  const int k = (int)whole, half = k / 2;  // in two steps, since 2^k may be out of range where 2^x is not
+  return (double)exp2f((float)(x - whole)) * __hiloint2double((1023 + half) << 20, 0) * __hiloint2double((1023 + k - half) << 20, 0);
+}
+
+// e^d - 1 for d in units of log 2.
+LZ_DEV double expm1_wide(double d2) {
+  return fabs(d2) < 1.0 ? (double)expm1f((float)(d2 * kLn2)) : exp2_wide(d2) - 1.0;
+}
 
 template <int KIND>
 LZ_DEV RowOut row_out(const LzLossArgs& a, const RowParams& p, const Norm& n, float c) {
   RowOut o;
   o.norm = n;
   o.logp2 = p.token < 0 ? (double)NAN : ((double)p.xy - (double)n.base) * (double)c - n.lse2;
-  o.ratio = 0.f, o.clipped = false, o.slope = KIND == LZ_LOSS_DISTILL ? p.slope : 0.f;
+  o.ratio = 0.0, o.clipped = false, o.slope = KIND == LZ_LOSS_DISTILL ? p.slope : 0.f;
   if (KIND == LZ_LOSS_POLICY) {
-    o.ratio = exp2f((float)(o.logp2 - p.old_logp2));
-    o.clipped = (p.adv > 0.f && o.ratio > 1.f + a.clip_high) || (p.adv < 0.f && o.ratio < 1.f - a.clip_low);
-    float slope = o.clipped ? 0.f : -p.adv * o.ratio;
-    if (a.kl_coef != 0.f) slope -= a.kl_coef * expm1f((float)((p.ref_logp2 - o.logp2) * kLn2));
-    o.slope = (float)(p.weight * (double)slope);
+    o.ratio = exp2_wide(o.logp2 - p.old_logp2);
+    o.clipped = (p.adv > 0.f && o.ratio > 1.0 + (double)a.clip_high) || (p.adv < 0.f && o.ratio < 1.0 - (double)a.clip_low);
+    double slope = o.clipped ? 0.0 : -(double)p.adv * o.ratio;
+    if (a.kl_coef != 0.f) slope -= (double)a.kl_coef * expm1_wide(p.ref_logp2 - o.logp2);
+    o.slope = (float)(p.weight * slope);
   }
   return o;
 }
@@ -431,7 +446,7 @@ LZ_DEV double row_write(const LzLossArgs& a, const RowParams& p, const RowOut& o
   double each = kl;
   if (KIND == LZ_LOSS_POLICY) {
     const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
-    each = -(double)p.adv * (o.clipped ? (p.adv > 0.f ? hi : lo) : (double)o.ratio);
+    each = -(double)p.adv * (o.clipped ? (p.adv > 0.f ? hi : lo) : o.ratio);
     if (a.ref_logp) {
       const double d = (p.ref_logp2 - o.logp2) * kLn2;
       kl = expm1(d) - fmin(d, DBL_MAX);  // +inf where the token has probability zero

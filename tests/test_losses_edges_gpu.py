@@ -139,3 +139,23 @@ def test_a_watched_kl_changes_nothing(v, low):
     for up in (1.0, 2.0):
         a, b = (torch.autograd.grad(o.loss, x, torch.tensor(up, device="cuda"), retain_graph=True)[0] for o in (out, plain))
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("v", [40, 1003, 40000])
+def test_scores_far_apart(v):
+    """Ratios and KL terms beyond fp32 that the advantage, the weight or the denominator brings back."""
+    x, y, old, _, ref = _policy_case(6, v, FP32, 1)
+    lp = oracle.logp64(x, y[:, None], 1.0)[0][:, 0]
+    old, ref = (lp - 0.1).float(), (lp + 0.1).float()
+    old[1], old[2], old[3], ref[4] = lp[1] - 100, lp[2] - 100, lp[3] + 200, lp[4] + 95
+    adv = torch.tensor([1.0, 0.0, -1e-3, -1.0, 0.0, 2.0], device="cuda")
+    z = x.requires_grad_(True)
+    out = lz.policy_loss(z, y, old, adv, weights=torch.tensor([1.0, 1, 0, 1, 1, 1], device="cuda"))
+    assert torch.isfinite(out.loss) and torch.isfinite(torch.autograd.grad(out.loss, z)[0]).all()
+    want = oracle.policy(x.detach(), y, old, adv, ref, None, 0.2, 0.25, 0.5, 1.0, 1e35)["kl"]
+    for upstream in (1.0, 2.0):
+        out = lz.policy_loss(z, y, old, adv, ref_logp=ref, clip_low=0.2, clip_high=0.25, kl_coef=0.5, denom=1e35)
+        grad, = torch.autograd.grad(out.loss, z, torch.tensor(upstream, device="cuda"))
+        assert (out.kl == math.inf).tolist() == [False] * 4 + [True, False]  # as a number of 32 bits
+        out = out._replace(kl=torch.where(out.kl.isinf(), want, out.kl.double()))
+        _check_policy(x.detach(), y, old, adv, ref, beta=0.5, denom=1e35, upstream=upstream, out=out, grad=grad)
