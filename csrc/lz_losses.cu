@@ -450,7 +450,8 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(const __grid_constant__ 
   for (int k = 0; k < 2; ++k)
     for (long long r = begin[k] + threadIdx.x; r < end[k]; r += kThreads)
       if (load_id(a.ids, a.ids64, r) >= 0) slope[r] = (float)((k ? -dh : dh) * per[k]);
-  if (threadIdx.x == 0) a.work[1 + pair] = (1.0 - a.smoothing) * up + a.smoothing * down;
+  // a term of weight zero is none, though an answer that cannot be makes it infinite
+  if (threadIdx.x == 0) a.work[1 + pair] = (a.smoothing < 1.0 ? (1.0 - a.smoothing) * up : 0.0) + (a.smoothing > 0.0 ? a.smoothing * down : 0.0);
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) last = atomicAdd(reinterpret_cast<unsigned*>(a.work), 1u) == gridDim.x - 1;

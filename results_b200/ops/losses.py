@@ -398,8 +398,9 @@ def _cpu_preference_loss(logits, tokens, ref, offsets, p):
         sums.append(logp[a:b].sum() / count)
     r = p["beta"] * (torch.stack(sums) - (0.0 if ref is None else ref.double()))
     h, eps = r[:pairs] - r[pairs:], p["label_smoothing"]
-    loss = -((1 - eps) * torch.nn.functional.logsigmoid(h) + eps * torch.nn.functional.logsigmoid(-h))
-    return loss.mean().float(), r.detach().float()
+    # a term of weight zero is none, though an answer that cannot be makes it infinite
+    terms = [-w * torch.nn.functional.logsigmoid(x) for w, x in ((1 - eps, h), (eps, -h)) if w]
+    return sum(terms).mean().float(), r.detach().float()
 
 
 # ---- public entry points ---------------------------------------------------------------------------------

@@ -78,3 +78,16 @@ def test_a_watched_kl_changes_nothing():
     assert torch.equal(out.loss, plain.loss) and torch.isfinite(out.loss) and torch.all(out.kl[1:3] == math.inf)
     a, b = (torch.autograd.grad(o.loss, x)[0] for o in (out, plain))
     assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("side", [0, 1])
+def test_preference_with_an_impossible_token(side):
+    x, y, _ = _inputs(4, 8)
+    with torch.no_grad():
+        x[2 * side, y[2 * side]] = -math.inf
+    for eps in (0.0, 1.0):
+        out = lz.preference_loss(x.view(2, 2, 8), y.view(2, 2), label_smoothing=eps)
+        zero = side == (1 if eps == 0.0 else 0)
+        assert float(out.loss.detach()) == (0.0 if zero else math.inf)
+        grad, = torch.autograd.grad(out.loss, x)
+        assert torch.isfinite(grad).all() and bool((grad == 0).all()) == zero

@@ -159,3 +159,20 @@ def test_scores_far_apart(v):
         assert (out.kl == math.inf).tolist() == [False] * 4 + [True, False]  # as a number of 32 bits
         out = out._replace(kl=torch.where(out.kl.isinf(), want, out.kl.double()))
         _check_policy(x.detach(), y, old, adv, ref, beta=0.5, denom=1e35, upstream=upstream, out=out, grad=grad)
+
+
+@pytest.mark.parametrize("v", [40, 40000])
+@pytest.mark.parametrize("side", [0, 1])
+def test_preference_with_an_impossible_token(v, side):
+    """A token of probability zero in one answer: the margin is infinite. Without smoothing the loss has one
+    term, which is zero (a rejected answer that cannot be) or infinite."""
+    x = _logits(4, v, FP32, 1)
+    y = _tokens(4, v, 2)
+    x[2 * side, y[2 * side]] = -math.inf
+    x.requires_grad_(True)
+    for eps in (0.0, 1.0):
+        out = lz.preference_loss(x.view(2, 2, v), y.view(2, 2), label_smoothing=eps)
+        zero = side == (1 if eps == 0.0 else 0)
+        assert float(out.loss.detach()) == (0.0 if zero else math.inf)
+        grad, = torch.autograd.grad(out.loss, x)
+        assert torch.isfinite(grad).all() and bool((grad == 0).all()) == zero
