@@ -229,7 +229,7 @@ class _Call:
     def forward(self) -> None:
         _launch("lz_loss_forward", self.args, _NAMES[self.args.kind])
 
-    def set_upstream(self, a, g: int, saved) -> None:
+    def set_upstream(self, a, g: int, rest) -> None:
         """`g`: address of the upstream gradient, of each row's log-probability or of the loss."""
         if a.kind == LOGP:
             a.row_upstream = g
@@ -243,17 +243,23 @@ class _Call:
         grad = self.__dict__.pop("grad", None)
         if g.dtype is not torch.float32 or not g.is_contiguous():
             g = g.to(torch.float32).contiguous()
-        if x.data_ptr() != a.logits:  # a saved tensor that came back from elsewhere
-            x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(x)
-            a.logits = x.data_ptr()
-        a.ids, a.work = saved[1].data_ptr(), saved[2].data_ptr()
+        # Hooks on saved tensors may give back other ones, in other layouts, at any address.
+        for t, kept in zip(saved, self.kept):
+            if t.get_device() != a.device or (t.dtype, t.shape) != kept:
+                raise RuntimeError(f"{_NAMES[a.kind]}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}; "
+                                   f"expected {kept[0]} {tuple(kept[1])} on cuda:{a.device}")
+        x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(x)
+        rest = [t.contiguous() for t in saved[1:]]
+        if rest[1].data_ptr() % 16:
+            rest[1] = rest[1].clone()
+        a.logits, a.ids, a.work = x.data_ptr(), rest[0].data_ptr(), rest[1].data_ptr()
         if a.kind == DISTILL:
-            a.teacher = saved[3].data_ptr()
+            a.teacher = rest[2].data_ptr()
         if grad is None:
             a.fresh = 1
             grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
             a.grad = grad.data_ptr()
-        self.set_upstream(a, g.data_ptr(), saved)
+        self.set_upstream(a, g.data_ptr(), rest)
         _launch("lz_loss_backward", a, _NAMES[a.kind])
         return grad
 
@@ -263,6 +269,7 @@ class _Loss(torch.autograd.Function):
     def forward(ctx, logits, call):
         call.forward()
         ctx.save_for_backward(*call.keep)
+        call.kept = [(t.dtype, t.shape) for t in call.keep]
         ctx.call, out = call, call.out
         call.keep = call.out = None  # the output leads here: it may not be held from here
         return out
@@ -308,8 +315,8 @@ class _PairsCall(_Call):
         _launch("lz_loss_pairs", self.pairs, "preference loss")
         self.alive = None
 
-    def set_upstream(self, a, g: int, saved) -> None:
-        a.upstream, a.row_upstream = g, saved[3].data_ptr() + self.slopes
+    def set_upstream(self, a, g: int, rest) -> None:
+        a.upstream, a.row_upstream = g, rest[2].data_ptr() + self.slopes
 
 
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------

@@ -176,3 +176,72 @@ def test_preference_with_an_impossible_token(v, side):
         assert float(out.loss.detach()) == (0.0 if zero else math.inf)
         grad, = torch.autograd.grad(out.loss, x)
         assert torch.isfinite(grad).all() and bool((grad == 0).all()) == zero
+
+
+@pytest.mark.parametrize("v", [301, 40000])
+def test_saved_logits_may_come_back_in_another_layout(v):
+    """Offloaded logits that come back contiguous, to the address that their strided view had."""
+    y = _tokens(12, v, 2).view(3, 4)
+    old, adv = torch.randn(2, 3, 4, device="cuda", generator=_gen(3)) - 5
+    ids = torch.randint(0, v, (3, 4, 5), device="cuda", generator=_gen(4))
+    t = torch.randn(3, 4, 5, device="cuda", generator=_gen(5))
+    store = _logits(15, v, BF16, 1).view(3, 5, v)
+
+    def step(hooked):
+        base = store.clone().requires_grad_(True)
+        z = base * 1  # not a leaf: only the view below is kept
+        view = z[:, :-1]
+        if not hooked:
+            return base, view, None
+
+        def pack(s):
+            return s.contiguous().clone(), s.data_ptr() == view.data_ptr() and s.dim() == 3
+
+        def unpack(p):
+            if not p[1]:
+                return p[0].clone()
+            flat = z.detach().view(-1)[:p[0].numel()].view(p[0].shape)
+            assert flat.data_ptr() == view.data_ptr()
+            return flat.copy_(p[0])
+
+        return base, view, torch.autograd.graph.saved_tensors_hooks(pack, unpack)
+
+    for f in (lambda x: lz.policy_loss(x, y, old, adv).loss, lambda x: lz.distill_loss(x, ids, t).loss,
+              lambda x: lz.token_logprobs(x, y).sum(),
+              lambda x: lz.preference_loss(x[:2], y[:2]).loss):
+        grads = []
+        for hooked in (False, True):
+            base, view, hooks = step(hooked)
+            if hooks:
+                with hooks:
+                    loss = f(view) * 3
+            else:
+                loss = f(view) * 3
+            grads += torch.autograd.grad(loss, base)
+        assert torch.equal(*grads)
+
+
+def test_saved_tensors_may_come_back_with_other_strides():
+    """Tokens and lists that are not contiguous any more; a tensor that stays on the host is refused."""
+    x, ids, t = _distill_case(6, 1003, 5, BF16, 3)
+    y = ids[:, 0].contiguous()
+    x.requires_grad_(True)
+
+    def spread(s):
+        wide = torch.zeros(*s.shape, 2, dtype=s.dtype, device=s.device)
+        wide[..., 0] = s.detach()
+        return wide[..., 0]
+
+    def shift(s):  # behind one element of a buffer
+        return torch.cat([s.detach().reshape(-1)[:1], s.detach().reshape(-1)])[1:].view(s.shape)
+
+    for f in (lambda: lz.token_logprobs(x, y).sum(), lambda: lz.distill_loss(x, ids, t).loss):
+        want, = torch.autograd.grad(f() * 2, x)
+        for pack in (spread, shift):
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda s: s):
+                loss = f() * 2
+            assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s.cpu(), lambda s: s):
+            loss = f() * 2
+        with pytest.raises(RuntimeError, match="saved"):
+            torch.autograd.grad(loss, x)
