@@ -576,7 +576,18 @@ int run_kind(const LzLossArgs* a, cudaStream_t s, bool forward) {
   }
 }
 
-int run(const LzLossArgs* a, cudaStream_t s, bool forward) {
+// The id of the graph capture that the stream is in, 0 for none.
+unsigned long long capture_of(cudaStream_t s) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream while another one is captured: not in a capture itself
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
+int run(LzLossArgs* a, cudaStream_t s, bool forward) {
   if (a->kind < LZ_LOSS_LOGP || a->kind > LZ_LOSS_DISTILL || a->rows < 0 || a->vocab < 1 || a->vocab > INT32_MAX ||
       a->inner < 1 || a->inv_temperature <= 0.f ||
       (a->kind == LZ_LOSS_DISTILL && (a->top < 1 || a->top > LZ_LOSS_MAX_TOP))) {
@@ -585,6 +596,8 @@ int run(const LzLossArgs* a, cudaStream_t s, bool forward) {
   }
   const OnDevice on(a->device);
   LZ_CUDA_TRY(on.rc);
+  if (forward) a->capture = capture_of(s);
+  else if (!a->fresh && a->capture != capture_of(s)) return LZ_LOSS_APART;
   switch (a->dtype) {
     case LZ_F32: return run_kind<float>(a, s, forward);
     case LZ_F16: return run_kind<__half>(a, s, forward);
@@ -596,7 +609,7 @@ int run(const LzLossArgs* a, cudaStream_t s, bool forward) {
 
 }  // namespace
 
-extern "C" int lz_loss_forward(const LzLossArgs* a, cudaStream_t stream) { return run(a, stream, true); }
+extern "C" int lz_loss_forward(LzLossArgs* a, cudaStream_t stream) { return run(a, stream, true); }
 
 extern "C" int lz_loss_backward(const LzLossArgs* a, cudaStream_t stream) {
   // What only the forward pass reads may be gone by now.

@@ -48,11 +48,17 @@ struct LzLossArgs {
   float inv_temperature, clip_low, clip_high, kl_coef;
   int kind, dtype, ids64, top, teacher_dtype, device;
   int fresh;             // backward: 1 when `grad` does not hold the gradient for upstream 1 yet
+  unsigned long long capture;  // of the forward pass (set by it): the id of the graph capture that it ran in, 0 for none
 };
 
+#define LZ_LOSS_APART 1  /* nothing ran: the forward pass ran in another capture */
+
 // Statistics, outputs and (grad != null) the gradient for upstream 1.
-int lz_loss_forward(const struct LzLossArgs* a, cudaStream_t stream);
-// The gradient for another upstream value, from the statistics in `work`.
+int lz_loss_forward(struct LzLossArgs* a, cudaStream_t stream);
+// The gradient for another upstream value, from the statistics in `work`. Without `fresh` it
+// returns LZ_LOSS_APART where one of the two passes can run again without the other (either was
+// captured into a graph, or each into one of its own): `grad` is then the wrong memory to hand out,
+// since it is only written for upstream 1 by the forward pass, and any time that runs again.
 int lz_loss_backward(const struct LzLossArgs* a, cudaStream_t stream);
 
 // Preference loss from the rows' log-probabilities (the `work` that lz_loss_forward

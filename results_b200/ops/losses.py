@@ -23,9 +23,11 @@ forward pass, while a row is still on the chip, for an upstream gradient of 1;
 the backward pass looks at the upstream on the device and computes the
 gradient anew, from the logits, if it is another (a loss divided by the number
 of micro batches, a loss scaler). Pass such a factor through ``denom`` instead
-to keep the cheaper way. The logits must not be changed before the backward
-pass. CUDA tensors run the kernels in csrc/lz_losses.cu on the current stream
-of their device; CPU tensors run the definitions in 64-bit torch operations.
+to keep the cheaper way, and capture both passes into one CUDA graph: a backward
+pass captured apart computes the gradient anew at every replay. The logits must
+not be changed before the backward pass. CUDA tensors run the kernels in
+csrc/lz_losses.cu on the current stream of their device; CPU tensors run the
+definitions in 64-bit torch operations.
 """
 from __future__ import annotations
 
@@ -55,7 +57,7 @@ class _LossArgs(C.Structure):  # struct LzLossArgs
                 ("weights", _p), ("denom_ptr", _p), ("upstream", _p), ("row_upstream", _p), ("loss", _p), ("logp", _p),
                 ("kl", _p), ("clipped", _p), ("work", _p), ("denom", _d), ("inv_temperature", _f), ("clip_low", _f),
                 ("clip_high", _f), ("kl_coef", _f), ("kind", _i), ("dtype", _i), ("ids64", _i), ("top", _i),
-                ("teacher_dtype", _i), ("device", _i), ("fresh", _i)]
+                ("teacher_dtype", _i), ("device", _i), ("fresh", _i), ("capture", C.c_ulonglong)]
 
 
 class _PairArgs(C.Structure):  # struct LzPairArgs
@@ -185,13 +187,18 @@ def _rows_of(x: torch.Tensor):
 _lib = None
 
 
-def _launch(fn: str, a, what: str) -> None:
+_APART = 1  # LZ_LOSS_APART
+
+
+def _launch(fn: str, a, what: str) -> bool:
+    """False: nothing ran, the forward pass belongs to another graph capture."""
     global _lib
     if _lib is None:
         _lib = _native.cuda()
     rc = getattr(_lib, fn)(C.byref(a), torch._C._cuda_getCurrentRawStream(a.device))
-    if rc:
+    if rc and rc != _APART:
         _native.check(rc, what)
+    return not rc
 
 
 class _Call:
@@ -238,7 +245,8 @@ class _Call:
 
     def backward(self, saved, g) -> torch.Tensor:
         """The gradient is handed out once: a second pass over a retained graph
-        writes into memory of its own."""
+        writes into memory of its own, and so does a pass that was captured
+        apart from the forward pass."""
         a, x = _LossArgs.from_buffer_copy(self.args), saved[0]  # other threads may be here too
         grad = self.__dict__.pop("grad", None)
         if g.dtype is not torch.float32 or not g.is_contiguous():
@@ -255,12 +263,12 @@ class _Call:
         a.logits, a.ids, a.work = x.data_ptr(), rest[0].data_ptr(), rest[1].data_ptr()
         if a.kind == DISTILL:
             a.teacher = rest[2].data_ptr()
-        if grad is None:
+        self.set_upstream(a, g.data_ptr(), rest)
+        if grad is None or not _launch("lz_loss_backward", a, _NAMES[a.kind]):
             a.fresh = 1
             grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
             a.grad = grad.data_ptr()
-        self.set_upstream(a, g.data_ptr(), rest)
-        _launch("lz_loss_backward", a, _NAMES[a.kind])
+            _launch("lz_loss_backward", a, _NAMES[a.kind])
         return grad
 
 

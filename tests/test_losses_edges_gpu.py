@@ -245,3 +245,55 @@ def test_saved_tensors_may_come_back_with_other_strides():
             loss = f() * 2
         with pytest.raises(RuntimeError, match="saved"):
             torch.autograd.grad(loss, x)
+
+
+@pytest.mark.parametrize("v", [700, 40000])
+@pytest.mark.parametrize("kind", ["policy", "distill"])
+def test_backward_captured_apart(v, kind):
+    """A backward pass in a graph of its own gives the formula's gradient at every replay, whatever was done to
+    the last one and whatever upstream that had; its forward pass ran eagerly or in another graph."""
+    x, y, old, adv, ref = _policy_case(12, v, BF16, 2)
+    x, ids, t = _distill_case(12, v, 9, BF16, 2)
+    x.requires_grad_(True)
+
+    def f():
+        if kind == "policy":
+            return lz.policy_loss(x, y, old, adv, ref_logp=ref, kl_coef=0.1).loss
+        return lz.distill_loss(x, ids, t).loss
+
+    want = {u: torch.autograd.grad(f(), x, torch.tensor(u, device="cuda"))[0] for u in (1.0, 2.0)}
+    for captured in (False, True):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # a pass before the capture, as every graph has it
+            torch.autograd.grad(f(), x)
+            if not captured:
+                loss = f()
+        torch.cuda.current_stream().wait_stream(side)
+        if captured:
+            first = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(first, stream=side):
+                loss = f()
+            first.replay()
+        up = torch.ones((), device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            grad, = torch.autograd.grad(loss, x, up, retain_graph=True)
+            half = grad * 0.5
+            grad.mul_(4)
+        for u in (1.0, 2.0, 1.0, 1.0):
+            up.fill_(u)
+            graph.replay()
+            assert torch.equal(grad, want[u] * 4) and torch.equal(half, want[u] * 0.5)
+    # and a captured forward pass with an eager backward pass: a replay writes over no gradient that was given out
+    first.replay()
+    first.replay()
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):
+        loss2 = f()
+    g2.replay()
+    a, = torch.autograd.grad(loss2, x, retain_graph=True)
+    a.zero_()
+    g2.replay()
+    assert torch.all(a == 0)
+    assert torch.equal(torch.autograd.grad(loss2, x)[0], want[1.0])
