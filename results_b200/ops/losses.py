@@ -26,8 +26,9 @@ of micro batches, a loss scaler). Pass such a factor through ``denom`` instead
 to keep the cheaper way, and capture both passes into one CUDA graph: a backward
 pass captured apart computes the gradient anew at every replay. The logits must
 not be changed before the backward pass. CUDA tensors run the kernels in
-csrc/lz_losses.cu on the current stream of their device; CPU tensors run the
-definitions in 64-bit torch operations.
+csrc/lz_losses.cu on the current stream of their device, with a first derivative
+in the logits by the backward pass (no second one, no forward mode, no tracing);
+CPU tensors run the definitions in 64-bit torch operations.
 """
 from __future__ import annotations
 
@@ -36,6 +37,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native, _native_sigs
 from ..utils.dtypes import LZ_BF16, LZ_F16, LZ_F32
@@ -155,6 +157,16 @@ def _check_denom(what: str, denom, device):
     if denom.requires_grad:
         raise ValueError(f"{what}: denom requires a gradient, and this loss gives none to it; detach it")
     return denom.to(torch.float32)
+
+
+def _check_modes(what: str, *tensors: torch.Tensor | None) -> None:
+    """CUDA tensors: what goes past autograd functions would be lost in the kernels."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what}: a call with CUDA tensors cannot be traced")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}: no forward-mode derivative for CUDA tensors")
 
 
 # ---- native calls ---------------------------------------------------------------------------------------
@@ -434,6 +446,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     temperature = _check_temperature(what, temperature)
     if not logits.is_cuda:
         return _cpu_token_logprobs(logits, tokens, temperature)
+    _check_modes(what, logits)
     logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
     return _run(_Call(LOGP, logits, tokens, temperature, logp, logp), logits, _needs_grad(logits))
 
@@ -470,6 +483,7 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
          "temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
     if not logits.is_cuda:
         return PolicyLoss(*_cpu_policy_loss(logits, tokens, rows, p))
+    _check_modes(what, logits, old_logp, advantages, ref_logp, weights, denom)
     needs_grad, old = _needs_grad(logits), rows[0]  # old_logp: contiguous, fp32, of the tokens' shape
     logp, clipped = torch.empty_like(old), torch.empty_like(old, dtype=torch.bool)
     kl = None if ref_logp is None else torch.empty_like(old)
@@ -516,6 +530,7 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, *, ref_logp: tor
     if not logits.is_cuda:
         loss, rewards = _cpu_preference_loss(logits, tokens, ref, cu_seqlens, p)
     else:
+        _check_modes(what, logits, ref_logp)
         call = _PairsCall(logits, tokens, ref, cu_seqlens, p)
         loss, rewards = _run(call, logits, _needs_grad(logits)), call.rewards
     return PreferenceLoss(loss, *rewards.split(p["pairs"]))
@@ -553,6 +568,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     p = {"temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
     if not logits.is_cuda:
         return DistillLoss(*_cpu_distill_loss(logits, ids, teacher, weights, p))
+    _check_modes(what, logits, teacher_logits, weights, denom)
     needs_grad = _needs_grad(logits)
     kl = torch.empty(shape, dtype=torch.float32, device=dev)
     call = _Call(DISTILL, logits, ids, p["temperature"], kl.new_empty(()), None, kl, None, (None, None, None, weights), teacher,

@@ -297,3 +297,26 @@ def test_backward_captured_apart(v, kind):
     g2.replay()
     assert torch.all(a == 0)
     assert torch.equal(torch.autograd.grad(loss2, x)[0], want[1.0])
+
+
+def test_forward_mode_and_tracing_are_refused():
+    """Neither a tangent nor a recorded graph is lost without a word."""
+    from torch.autograd import forward_ad
+
+    x, ids, t = _distill_case(4, 300, 5, FP32, 3)
+    y = ids[:, 0].contiguous()
+    z = torch.zeros(4, device="cuda")
+    calls = [lambda x, z: lz.token_logprobs(x, y), lambda x, z: lz.policy_loss(x, y, z, z + 1).loss,
+             lambda x, z: lz.preference_loss(x.view(2, 2, 300), y.view(2, 2)).loss,
+             lambda x, z: lz.distill_loss(x, ids, t, weights=z + 1).loss]
+    for f in calls:
+        for needs_grad in (False, True):
+            leaf = x.clone().requires_grad_(needs_grad)
+            with forward_ad.dual_level():
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(forward_ad.make_dual(leaf, torch.ones_like(x)), z)
+                assert torch.equal(f(leaf, z), f(leaf, z))  # nothing to lose: as ever
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(lambda a: f(a, z), (leaf,), check_trace=False)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        calls[1](x, forward_ad.make_dual(z, torch.ones_like(z)))
