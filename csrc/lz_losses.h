@@ -49,6 +49,7 @@ struct LzLossArgs {
   int kind, dtype, ids64, top, teacher_dtype, device;
   int fresh;             // backward: 1 when `grad` does not hold the gradient for upstream 1 yet
   unsigned long long capture;  // of the forward pass (set by it): the id of the graph capture that it ran in, 0 for none
+  unsigned long long wait_ns;  // bound of every wait in the kernels; 0: 4 s, 1: nothing is waited for
 };
 
 #define LZ_LOSS_APART 1  /* nothing ran: the forward pass ran in another capture */

@@ -671,6 +671,7 @@ struct LzStreamPlan {
   int hash;     // entries of a hash table of DISTILL, a power of two; 0 where the list is short
   int views;    // DISTILL: rows whose lists are kept, 2 or 4
   size_t smem;
+  unsigned long long wait_ns;
 };
 int lz_stream_plan(const LzLossArgs* a, LzStreamPlan* plan);
 int lz_stream_forward(const LzLossArgs* a, const LzStreamPlan* plan, cudaStream_t stream);

@@ -20,7 +20,7 @@
 namespace {
 
 constexpr int kMaxSlots = 64;
-constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of every wait
+constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of every wait where the caller gives none
 
 // Which row, and this CTA's slice of it.
 struct RowHead {
@@ -69,9 +69,11 @@ LZ_DEV void mbar_expect(uint64_t* bar, uint32_t bytes) {
                : "memory");
 }
 
-// Waits for phase `parity` of `bar`, 4 s at most. A wait that gives up sets
-// `failed`, and the CTA's other waits then return at once: the kernel runs to its
-// end and leaves NaN.
+// Every wait for a phase of a barrier is bounded. One that gives up says so to all CTAs of
+// the cluster, whose other waits then give up at once unless their phase is there. Whoever
+// waited in vain leaves its loop without another look at what it waited for, arrives nowhere
+// and sends nothing, so what others still receive is right. When all threads have left,
+// every CTA of the cluster writes NaN over the outputs and gradients of the cluster's rows.
 template <bool CLUSTER>
 LZ_DEV bool try_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -94,26 +96,47 @@ LZ_DEV bool try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
+LZ_DEV void give_up(volatile int* failed) {
+  *failed = 1;
+  const uint32_t own = smem_addr(const_cast<int*>(failed)), ranks = cluster_size();
+  for (uint32_t rank = 0; ranks > 1 && rank < ranks; ++rank)
+    asm volatile(
+        "{\n\t.reg .b32 p;\n\t"
+        "mapa.shared::cluster.u32 p, %0, %1;\n\t"
+        "st.shared::cluster.u32 [p], 1;\n\t}" ::"r"(own),
+        "r"(rank)
+        : "memory");
+}
+
 template <bool CLUSTER>
-__device__ __noinline__ void ring_wait_on(uint32_t bar, uint32_t parity, volatile int* failed) {
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* failed, unsigned long long limit) {
   unsigned long long began = 0;
-  for (uint32_t it = 1; it; ++it) {
-    if (try_wait<CLUSTER>(bar, parity) || *failed) return;
+  for (uint32_t it = 1; it && limit > 1; ++it) {  // 1: what is not there at once is given up
+    if (try_wait<CLUSTER>(bar, parity)) return true;
+    if (*failed) return false;
     if (it % 64 == 0) {
       const unsigned long long now = globaltimer();
       if (!began) began = now;
-      if (now - began > kWaitNs) break;
+      if (now - began > limit) break;
     }
   }
-  *failed = 1;
+  give_up(failed);
+  return false;
 }
 
+// By one lane.
+LZ_DEV bool lane_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned long long limit) {
+  return try_wait<false>(smem_addr(bar), parity) || wait_on<false>(smem_addr(bar), parity, failed, limit);
+}
+
+// By a whole warp; the same in every lane.
 template <bool CLUSTER>
-LZ_DEV void ring_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  if (!try_wait<CLUSTER>(smem_addr(bar), parity)) ring_wait_on<CLUSTER>(smem_addr(bar), parity, failed);
+LZ_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned long long limit) {
+  if (__all_sync(~0u, try_wait<CLUSTER>(smem_addr(bar), parity))) return true;
+  return __all_sync(~0u, wait_on<CLUSTER>(smem_addr(bar), parity, failed, limit));
 }
 
-// After a wait that gave up: copies still in flight land before the CTA ends.
+// After a wait that gave up: copies and peers' values still in flight land before the CTA ends.
 LZ_DEV void drain_copies() {
   const unsigned long long began = globaltimer();
   for (uint32_t it = 0; it < 100000000u && globaltimer() - began < 20000000ull; ++it) {
@@ -155,6 +178,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
   const long long cluster = blockIdx.x / ranks, clusters = gridDim.x / ranks;
   const float c = (float)(kLog2e * (double)a.inv_temperature);
   volatile int* const failed = &sh.failed;
+  const unsigned long long limit_ns = plan.wait_ns;
   // Rows of this cluster: i = cluster, cluster + clusters, ... below `limit`, those that count first.
   const long long limit = plan.ordered ? a.rows : min(a.rows, clusters);
   const int active = plan.ordered ? *work_active(a) : 0;
@@ -201,16 +225,15 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       for (long long i = cluster; h.row >= 0; i += clusters) {
         const RowHead next = head_at(i + clusters);
         const char* from = reinterpret_cast<const char*>(row_of<T>(a, h.row) + h.lead) + (size_t)h.first * 16;
-        for (int k = 0; k < h.chunks && !*failed; ++k) {
-          if (round) ring_wait<false>(&sh.empty[slot], (round - 1) & 1, failed);
-          if (*failed) break;
+        for (int k = 0; k < h.chunks; ++k) {
+          if (round && !lane_wait(&sh.empty[slot], (round - 1) & 1, failed, limit_ns)) goto fed;
           const int vecs = min(kChunkVecs, h.count - k * kChunkVecs);
           bulk_g2s(ring + (size_t)slot * kChunk, from + (size_t)k * kChunk, vecs * 16, &sh.full[slot]);
           if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
         }
         h = next;
       }
-      if (*failed) drain_copies();
+    fed:;
     }
     __syncwarp();
   } else if (warp < W) {  // ---- sums, then the dense gradient
@@ -219,11 +242,11 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     LazySum sum;
     sum.init(c);
     int done = 0;  // chunks of the row that are in `sum`
-    // Chunks [done, upto) of a row.
+    // Chunks [done, upto) of a row; false where one did not come.
     auto take = [&](const RowHead& h, int upto) {
       for (; done < upto; ++done) {
         const int vecs = h.count - done * kChunkVecs;
-        ring_wait<false>(&sh.full[slot], round & 1, failed);
+        if (!warp_wait<false>(&sh.full[slot], round & 1, failed, limit_ns)) return false;
         const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk) + tid;
         if (vecs >= kChunkVecs) {
           uint4 w[kBatch];
@@ -239,18 +262,20 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         }
         if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
       }
+      return true;
     };
     uint32_t turn = 0;
+    bool all_there = true;
     for (;; ++turn) {
       // The row's head is there, and its place in `warp_part` free, when the row two before it is done with.
       const int k = turn & 1;
-      if (!GRAD && turn >= 2) ring_wait<false>(&sh.dense[k], ((turn - 2) >> 1) & 1, failed);
+      if (!GRAD && turn >= 2 && !(all_there = warp_wait<false>(&sh.dense[k], ((turn - 2) >> 1) & 1, failed, limit_ns))) break;
       const RowHead h = sh.heads[turn & 3];
       if (h.row < 0) break;
       const long long single = rank == 0 && tid < 2 * N ? single_of(h.lead, h.vecs, N, tid, a.vocab) : -1;
       float alone = 0.f;
       if (single >= 0) alone = Elem<T>::get(row_of<T>(a, h.row)[single]);
-      take(h, h.chunks);
+      if (!(all_there = take(h, h.chunks))) break;
       if (single >= 0) sum.take_one(alone, c);
       float m = sum.ref, all = sum.total();
       lanes_join(m, all, 32);
@@ -262,8 +287,8 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       done = 0;
       if (!GRAD) continue;
       const RowHead& next = sh.heads[(turn + 1) & 3];
-      if (next.row >= 0) take(next, min(plan.early, next.chunks));
-      ring_wait<false>(&sh.dense[k], (turn >> 1) & 1, failed);
+      if (next.row >= 0 && !(all_there = take(next, min(plan.early, next.chunks)))) break;
+      if (!(all_there = warp_wait<false>(&sh.dense[k], (turn >> 1) & 1, failed, limit_ns))) break;
       const RowGrad d = sh.grad[k];
       T* out = static_cast<T*>(a.grad) + h.row * a.vocab;
       const uint64_t c2 = pair(c, c), f2 = pair(d.f, d.f), off2 = pair(-d.ref, -d.ref);
@@ -303,7 +328,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         out[single] = Elem<T>::put(d.f == 0.f ? 0.f : d.dense(alone, c));
     }
     __syncwarp();
-    if (GRAD) {
+    if (GRAD && all_there) {
       if (lane == 0) mbar_arrive(&sh.parts[turn & 1]);  // the last row is written
       for (long long i = (plan.ordered ? active : 0) + cluster; i < limit; i += clusters) {
         long long r;
@@ -323,7 +348,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     for (uint32_t turn = mine; mine < views / 2 && row_at(cluster + (long long)turn * clusters, &r); turn += views / 2) {
       const int k = turn & (views - 1);
       if (row_at(cluster + (long long)(turn + views) * clusters, &to_come)) touch_list(a, to_come);
-      if (turn >= views) ring_wait<false>(&sh.used[k], ((turn >> views_log2) - 1) & 1, failed);
+      if (turn >= views && !warp_wait<false>(&sh.used[k], ((turn >> views_log2) - 1) & 1, failed, limit_ns)) break;
       prepare_params<T, KIND>(a, row_of<T>(a, r), r, sh.params[k], view(k), hash, plan.hash, c);
       if (lane == 0) mbar_arrive(&sh.ready[k]);
       if (row_at(cluster + (long long)(turn + views / 2) * clusters, &to_come))
@@ -359,25 +384,26 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     };
     prepare(sh.heads[0], 0);
     uint32_t turn = 0;
+    bool all_there = true;
     for (;; ++turn) {
       const RowHead h = sh.heads[turn & 3];
       if (h.row < 0) break;
       const int k = turn & 1, at = turn & (views - 1), last = (turn - 1) & (views - 1);
       const RowHead later = head_at(cluster + (long long)(turn + 2) * clusters);
-      ring_wait<false>(&sh.parts[k], (turn >> 1) & 1, failed);
+      if (!(all_there = warp_wait<false>(&sh.parts[k], (turn >> 1) & 1, failed, limit_ns))) break;
       float2 v = lane < W ? sh.warp_part[k][lane] : make_float2(-INFINITY, 0.f);
       lanes_join(v.x, v.y, W);
       if (ranks > 1) {
         if (lane == 0) mbar_expect(&sh.peers[k], ranks * (uint32_t)sizeof(float2));
         if (lane < ranks) send_to_peer(&sh.peer_part[k][rank], v, &sh.peers[k], lane);
         __syncwarp();
-        ring_wait<true>(&sh.peers[k], (turn >> 1) & 1, failed);
+        if (!(all_there = warp_wait<true>(&sh.peers[k], (turn >> 1) & 1, failed, limit_ns))) break;
         v = lane < ranks ? sh.peer_part[k][lane] : make_float2(-INFINITY, 0.f);
         lanes_join(v.x, v.y, kMaxCluster);
       }
       RowSum n = {0.f, v.x, v.y};
       if (!exact_ref(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
-      if (KIND == LZ_LOSS_DISTILL) ring_wait<false>(&sh.ready[at], (turn >> views_log2) & 1, failed);
+      if (KIND == LZ_LOSS_DISTILL && !(all_there = warp_wait<false>(&sh.ready[at], (turn >> views_log2) & 1, failed, limit_ns))) break;
       const RowParams& p = sh.params[at];
       const RowOut o = row_out<KIND>(a, p, n.norm(), c);
       const RowGrad g(o.slope, a.inv_temperature, n);
@@ -394,23 +420,14 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       __syncwarp();
       prepare(sh.heads[(turn + 1) & 3], k ^ 1);
     }
-    if (GRAD) {
-      ring_wait<false>(&sh.parts[turn & 1], (turn >> 1) & 1, failed);
+    if (GRAD && all_there && (all_there = warp_wait<false>(&sh.parts[turn & 1], (turn >> 1) & 1, failed, limit_ns)))
       sparse((turn - 1) & (views - 1));
-    }
     if (rank == 0) {
       long long r;
       for (long long i = (plan.ordered ? active : 0) + cluster + lane * clusters; i < limit; i += 32 * clusters) {
         if (!row_at(i, &r)) no_outputs<KIND>(a, r);
       }
-      if (*failed) {
-        loss = NAN;
-        for (long long i = cluster + lane * clusters; i < limit; i += 32 * clusters) {
-          row_at(i, &r);
-          if (KIND != LZ_LOSS_DISTILL) a.logp[r] = NAN;
-          if (KIND == LZ_LOSS_DISTILL || (KIND == LZ_LOSS_POLICY && a.ref_logp)) a.kl[r] = NAN;
-        }
-      }
+      if (!all_there) loss = NAN;
       if (KIND != LZ_LOSS_LOGP) {  // the cluster that is done last adds the losses up, in the clusters' order
         int last = 0;
         if (lane == 0) {
@@ -431,6 +448,24 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     __syncwarp();
   }
   cluster_sync();  // no CTA leaves while a peer may still write to it
+  if (!*failed) return;
+  drain_copies();
+  for (long long i = cluster; i < limit; i += clusters) {
+    long long r;
+    row_at(i, &r);
+    if (GRAD) {
+      T* out = static_cast<T*>(a.grad) + r * a.vocab;
+      const long long per = (a.vocab + ranks - 1) / ranks, end = min((rank + 1) * per, a.vocab);
+      for (long long j = rank * per + tid; j < end; j += blockDim.x) out[j] = Elem<T>::put(NAN);
+    }
+    if (rank == 0 && tid == 0) {
+      if (KIND != LZ_LOSS_DISTILL) a.logp[r] = NAN;
+      if (KIND == LZ_LOSS_DISTILL || (KIND == LZ_LOSS_POLICY && a.ref_logp)) a.kl[r] = NAN;
+      if (KIND == LZ_LOSS_POLICY) a.clipped[r] = 0;
+      work_sum(a)[r] = make_float4(0.f, 0.f, NAN, 0.f);  // the backward pass's too
+      work_slope(a)[r] = NAN;
+    }
+  }
 }
 
 // The gradient alone, for rows whose sums and slopes are known (LOGP, POLICY). A
@@ -454,7 +489,8 @@ struct alignas(128) GradShared {
 };
 
 template <typename T, int KIND, int W>
-__global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __grid_constant__ LzLossArgs a, int slots) {
+__global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __grid_constant__ LzLossArgs a, int slots,
+                                                                      unsigned long long limit_ns) {
   constexpr int N = Elem<T>::N, kTake = W * 32;
   constexpr int kChunkVecs = kBatch * kTake, kChunk = 16 * kChunkVecs;
   extern __shared__ __align__(128) char smem[];
@@ -508,30 +544,31 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
         }
         from = reinterpret_cast<const char*>(x + at);
       }
+      bool free = true;
       for (int l = 0; l < 32 && first + (long long)l * gridDim.x < all; ++l) {
         if (lane == l) {
-          if (round) ring_wait<false>(&sh.empty[slot], (round - 1) & 1, failed);
-          if (!*failed) {
+          free = !round || lane_wait(&sh.empty[slot], (round - 1) & 1, failed, limit_ns);
+          if (free) {
             sh.heads[slot] = h;
             if (h.f != 0.f && h.vecs > 0) bulk_g2s(ring + (size_t)slot * kChunk, from, h.vecs * 16, &sh.full[slot]);
             else mbar_arrive(&sh.full[slot]);  // nothing to read
           }
         }
-        __syncwarp();
+        free = __shfl_sync(~0u, free, l);
+        if (!free) break;
         if (++slot == (uint32_t)slots) slot = 0, ++round;
       }
+      if (!free) break;
     }
-    if (*failed) drain_copies();
-    __syncwarp();
   } else {
     uint32_t slot = 0, round = 0;
     for (long long g = blockIdx.x; g < all; g += gridDim.x) {
-      ring_wait<false>(&sh.full[slot], round & 1, failed);
+      if (!warp_wait<false>(&sh.full[slot], round & 1, failed, limit_ns)) break;
       const ChunkHead& h = sh.heads[slot];
       const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk) + tid;
       uint4* o = static_cast<uint4*>(h.out) + tid;
-      const int vecs = *failed ? 0 : h.vecs;
-      const float f = *failed ? 0.f : h.f, base = h.base, ref = h.ref;
+      const int vecs = h.vecs;
+      const float f = h.f, base = h.base, ref = h.ref;
       const int token_vec = h.token_vec;
       if (f == 0.f) {
 #pragma unroll
@@ -561,7 +598,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
         if (token_vec >= 0 && token_vec % kTake == tid)  // over its vector, by the thread that wrote it
           reinterpret_cast<T*>(static_cast<uint4*>(h.out) + token_vec)[h.token_at] = Elem<T>::put(h.token_value);
       }
-      if (h.singles && tid < h.lead + h.tail && !*failed) {
+      if (h.singles && tid < h.lead + h.tail) {
         const long long i = tid < h.lead ? tid : a.vocab - h.tail + tid - h.lead;
         float e = 0.f;
         if (f != 0.f) e = i == h.token ? h.token_value : f * exp2_fast(fmaf(Elem<T>::get(static_cast<const T*>(h.row)[i]) - base, c, -ref));
@@ -571,9 +608,21 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
       if (lane == 0) mbar_arrive(&sh.empty[slot]);
       if (++slot == (uint32_t)slots) slot = 0, ++round;
     }
-    if (*failed)  // a wait gave up: the gradient is NaN, not stale
-      for (long long i = tid; i < a.rows * a.vocab; i += kTake)
-        static_cast<T*>(a.grad)[i] = Elem<T>::put(NAN);
+  }
+  __syncthreads();
+  if (!*failed) return;
+  drain_copies();
+  for (long long g = blockIdx.x; g < all; g += gridDim.x) {  // this CTA's chunks are NaN, not stale
+    const long long r = g / per_row, piece = g % per_row;
+    T* out = static_cast<T*>(a.grad) + r * a.vocab;
+    const Split<T> sp(out, a.vocab);
+    const long long at = sp.lead + piece * kChunkVecs * N, end = min(at + (long long)kChunkVecs * N, sp.lead + (long long)sp.vecs * N);
+    for (long long j = at + tid; j < end; j += blockDim.x) out[j] = Elem<T>::put(NAN);
+    if (piece == 0)
+      for (long long t = tid; t < 2 * N; t += blockDim.x) {
+        const long long single = single_of(sp.lead, sp.vecs, N, (int)t, a.vocab);
+        if (single >= 0) out[single] = Elem<T>::put(NAN);
+      }
   }
 }
 
@@ -650,6 +699,7 @@ int plan_as(const LzLossArgs* a, LzStreamPlan* l) {
   l->views = part <= 128 * 1024 && (kSharedMax - four) / kChunk >= slots ? 4 : 2;
   const int fixed = l->views == 4 ? four : two;
   l->smem = fixed + (size_t)slots * kChunk;
+  l->wait_ns = a->wait_ns ? a->wait_ns : kWaitNs;
   return LZE_OK;
 }
 
@@ -679,7 +729,7 @@ int launch_stream_grad(const LzLossArgs* a, cudaStream_t s) {
   // writes (4096 rows of 151936 in bf16, half of them read: 408 us a step against 432).
   constexpr int slots = 4;
   static_assert(slots * kChunk + sizeof(GradShared) <= kSharedMax && slots <= kMaxSlots, "ring");
-  kernel<<<n, (kStreamWarps + 1) * 32, sizeof(GradShared) + (size_t)slots * kChunk, s>>>(*a, slots);
+  kernel<<<n, (kStreamWarps + 1) * 32, sizeof(GradShared) + (size_t)slots * kChunk, s>>>(*a, slots, a->wait_ns ? a->wait_ns : kWaitNs);
   LZ_CUDA_TRY(cudaGetLastError());
   return LZE_OK;
 }

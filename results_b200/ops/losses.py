@@ -59,7 +59,8 @@ class _LossArgs(C.Structure):  # struct LzLossArgs
                 ("weights", _p), ("denom_ptr", _p), ("upstream", _p), ("row_upstream", _p), ("loss", _p), ("logp", _p),
                 ("kl", _p), ("clipped", _p), ("work", _p), ("denom", _d), ("inv_temperature", _f), ("clip_low", _f),
                 ("clip_high", _f), ("kl_coef", _f), ("kind", _i), ("dtype", _i), ("ids64", _i), ("top", _i),
-                ("teacher_dtype", _i), ("device", _i), ("fresh", _i), ("capture", C.c_ulonglong)]
+                ("teacher_dtype", _i), ("device", _i), ("fresh", _i), ("capture", C.c_ulonglong),
+                ("wait_ns", C.c_ulonglong)]
 
 
 class _PairArgs(C.Structure):  # struct LzPairArgs
