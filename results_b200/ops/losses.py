@@ -198,7 +198,7 @@ def _rows_of(x: torch.Tensor):
 
 
 _lib = None
-
+_saved_hooks = torch._C._autograd._top_saved_tensors_default_hooks
 
 _APART = 1  # LZ_LOSS_APART
 
@@ -249,7 +249,7 @@ class _Call:
     def forward(self) -> None:
         _launch("lz_loss_forward", self.args, _NAMES[self.args.kind])
 
-    def set_upstream(self, a, g: int, rest) -> None:
+    def set_upstream(self, a, g: int, saved) -> None:
         """`g`: address of the upstream gradient, of each row's log-probability or of the loss."""
         if a.kind == LOGP:
             a.row_upstream = g
@@ -264,19 +264,11 @@ class _Call:
         grad = self.__dict__.pop("grad", None)
         if g.dtype is not torch.float32 or not g.is_contiguous():
             g = g.to(torch.float32).contiguous()
-        # Hooks on saved tensors may give back other ones, in other layouts, at any address.
-        for t, kept in zip(saved, self.kept):
-            if t.get_device() != a.device or (t.dtype, t.shape) != kept:
-                raise RuntimeError(f"{_NAMES[a.kind]}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}; "
-                                   f"expected {kept[0]} {tuple(kept[1])} on cuda:{a.device}")
-        x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(x)
-        rest = [t.contiguous() for t in saved[1:]]
-        if rest[1].data_ptr() % 16:
-            rest[1] = rest[1].clone()
-        a.logits, a.ids, a.work = x.data_ptr(), rest[0].data_ptr(), rest[1].data_ptr()
-        if a.kind == DISTILL:
-            a.teacher = rest[2].data_ptr()
-        self.set_upstream(a, g.data_ptr(), rest)
+        if self.hooked or x.data_ptr() != a.logits or x.stride() != self.strides or saved[1].data_ptr() != a.ids or \
+                saved[2].data_ptr() != a.work or (a.kind == DISTILL and saved[3].data_ptr() != a.teacher):
+            saved = self.came_back(a, saved)
+            x = saved[0]
+        self.set_upstream(a, g.data_ptr(), saved)
         if grad is None or not _launch("lz_loss_backward", a, _NAMES[a.kind]):
             a.fresh = 1
             grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
@@ -284,13 +276,32 @@ class _Call:
             _launch("lz_loss_backward", a, _NAMES[a.kind])
         return grad
 
+    def came_back(self, a, saved):
+        """Hooks on saved tensors may give back other ones, in other layouts, at any address:
+        those that the kernels read, with their addresses and strides in `a`."""
+        expected = [(a.dtype, a.rows * a.vocab), (torch.int64 if a.ids64 else torch.int32, a.rows * max(1, a.top)),
+                    (torch.float64, _HEAD + _PER_ROW * a.rows)]
+        if a.kind == DISTILL:
+            expected.append((a.teacher_dtype, a.rows * a.top))
+        for t, (dtype, n) in zip(saved, expected):
+            if t.get_device() != a.device or _DTYPES.get(t.dtype, t.dtype) != dtype or t.numel() != n:
+                raise RuntimeError(f"{_NAMES[a.kind]}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}")
+        x, a.outer_stride, a.inner_stride, a.inner, _ = _rows_of(saved[0].view(self.shape))
+        saved = [x, *(t.contiguous() for t in saved[1:])]
+        if saved[2].data_ptr() % 16:
+            saved[2] = saved[2].clone()
+        a.logits, a.ids, a.work = (t.data_ptr() for t in saved[:3])
+        if a.kind == DISTILL:
+            a.teacher = saved[3].data_ptr()
+        return saved
+
 
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call):
         call.forward()
         ctx.save_for_backward(*call.keep)
-        call.kept = [(t.dtype, t.shape) for t in call.keep]
+        call.strides, call.hooked = call.keep[0].stride(), _saved_hooks(True) is not None
         ctx.call, out = call, call.out
         call.keep = call.out = None  # the output leads here: it may not be held from here
         return out
@@ -336,8 +347,14 @@ class _PairsCall(_Call):
         _launch("lz_loss_pairs", self.pairs, "preference loss")
         self.alive = None
 
-    def set_upstream(self, a, g: int, rest) -> None:
-        a.upstream, a.row_upstream = g, rest[2].data_ptr() + self.slopes
+    def came_back(self, a, saved):
+        work = saved[3].contiguous()
+        if work.get_device() != a.device or work.dtype is not torch.float64 or work.numel() * 8 < self.slopes + 4 * a.rows:
+            raise RuntimeError(f"preference loss: a saved tensor came back as {work.dtype} {tuple(work.shape)} on {work.device}")
+        return [*super().came_back(a, saved[:3]), work]
+
+    def set_upstream(self, a, g: int, saved) -> None:
+        a.upstream, a.row_upstream = g, saved[3].data_ptr() + self.slopes
 
 
 # ---- the definitions (CPU tensors) -----------------------------------------------------------------------
