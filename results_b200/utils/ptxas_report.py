@@ -19,7 +19,9 @@ from .build import CSRC, NVCC, NVCC_FLAGS
 
 _ENTRY = re.compile(r"Compiling entry function '(\S+)'")
 _SPILL = re.compile(r"(\d+) bytes stack frame, (\d+) bytes spill stores, (\d+) bytes spill loads")
-_USED = re.compile(r"Used (\d+) registers.*?(\d+) bytes smem")
+_PROPERTIES = re.compile(r"Function properties for (\S+)")
+_USED = re.compile(r"Used (\d+) registers")
+_SMEM = re.compile(r"(\d+) bytes smem")  # not printed where a kernel has no static shared memory
 
 
 def _demangle(names: list[str]) -> list[str]:
@@ -35,21 +37,32 @@ def kernels(src: Path) -> list[dict]:
         cmd = [NVCC, *NVCC_FLAGS, "-diag-suppress=550", "-Xptxas", "-v", "-I", str(CSRC), "-c", str(src),
                "-o", str(Path(d) / "k.o")]
         txt = subprocess.run(cmd, capture_output=True, text=True).stderr
-    rows, cur = [], None
+    return parse(txt)
+
+
+def parse(txt: str) -> list[dict]:
+    """The kernels in ptxas's output."""
+    rows, cur, of = [], None, None
     for line in txt.splitlines():
         m = _ENTRY.search(line)
         if m:
             cur = {"mangled": m.group(1), "stack": 0, "spill_st": 0, "spill_ld": 0}
             continue
+        m = _PROPERTIES.search(line)
+        if m:  # of the kernel, or of a function that it calls
+            of = m.group(1)
+            continue
         m = _SPILL.search(line)
         if m and cur is not None:
-            cur["stack"], cur["spill_st"], cur["spill_ld"] = map(int, m.groups())
+            if of in (None, cur["mangled"]):
+                cur["stack"], cur["spill_st"], cur["spill_ld"] = map(int, m.groups())
             continue
         m = _USED.search(line)
         if m and cur is not None:
-            cur["regs"], cur["smem"] = int(m.group(1)), int(m.group(2))
+            smem = _SMEM.search(line)
+            cur["regs"], cur["smem"] = int(m.group(1)), int(smem.group(1)) if smem else 0
             rows.append(cur)
-            cur = None
+            cur = of = None
     for r, name in zip(rows, _demangle([r["mangled"] for r in rows])):
         r["name"] = re.sub(r"\(anonymous namespace\)::", "", name)
     return rows
