@@ -382,7 +382,7 @@ def _cpu_token_logp(logits, y, counted, temperature):
 
 def _cpu_scale(weights, counted, denom):
     w = counted.double() if weights is None else torch.where(counted, weights.reshape(-1).double(), 0.0)
-    d = w.sum() if denom is None else torch.as_tensor(denom, dtype=torch.float64).reshape(())
+    d = w.sum() if denom is None else torch.as_tensor(denom, dtype=torch.float64, device=w.device).reshape(())
     return torch.where(d <= 0, 0.0, w / d)
 
 
@@ -417,7 +417,7 @@ def _cpu_distill_loss(logits, ids, teacher, weights, p):
     ids, t = ids.reshape(n, k), teacher.reshape(n, k).double() / p["temperature"]
     there = ids >= 0
     t = torch.where(there, t, -math.inf)
-    counted = torch.ones(n, dtype=torch.bool) if weights is None else weights.reshape(-1) != 0
+    counted = torch.ones(n, dtype=torch.bool, device=logits.device) if weights is None else weights.reshape(-1) != 0
     some = t.amax(1) != -math.inf
     logq = torch.log_softmax(torch.where(some[:, None], t, 0.0), 1)
     q = torch.where(there & some[:, None], logq.exp(), 0.0)
@@ -437,7 +437,7 @@ def _cpu_preference_loss(logits, tokens, ref, offsets, p):
     sums = []
     for a, b in zip(ends, ends[1:]):
         if not 0 <= a <= b <= y.numel():
-            sums.append(torch.tensor(math.nan, dtype=torch.float64))
+            sums.append(logp.new_tensor(math.nan))
             continue
         count = max(1, int((y[a:b] >= 0).sum())) if p["length_normalized"] else 1
         sums.append(logp[a:b].sum() / count)

@@ -91,3 +91,25 @@ def test_preference_with_an_impossible_token(side):
         assert float(out.loss.detach()) == (0.0 if zero else math.inf)
         grad, = torch.autograd.grad(out.loss, x)
         assert torch.isfinite(grad).all() and bool((grad == 0).all()) == zero
+
+
+def test_a_default_device_of_another_kind():
+    """Tensors go by the logits' device, whatever torch's default is."""
+    x, y, z = _inputs(6, 8)
+    y[1] = 8
+    w = torch.tensor([1.0, 0, 1, 1, 1, 1])
+    cu, ids, t = torch.tensor([0, 3, 2, 4, 5]), y.clamp(max=7)[:, None], torch.zeros(6, 1)
+
+    def run():
+        outs = [lz.token_logprobs(x, y), lz.policy_loss(x, y, z, z + 1, ref_logp=z, weights=w, denom=4.0).loss,
+                lz.distill_loss(x, ids, t).loss, lz.preference_loss(x, y, cu_seqlens=cu).loss]
+        return [o.detach() for o in outs] + [torch.autograd.grad(o.nan_to_num().sum(), x)[0] for o in outs]
+
+    want = run()
+    torch.set_default_device("meta")
+    try:
+        got = run()
+    finally:
+        torch.set_default_device(None)
+    for a, b in zip(want, got):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
