@@ -366,3 +366,28 @@ def test_waits_that_give_up(monkeypatch, wait_ns, n, v, dtype):
             if k in ("policy", "distill"):
                 assert torch.equal(fused.isnan().all(1), fused.isnan().any(1)) and fused[lost].isnan().all()
             assert other[lost & counted].isnan().all()
+
+
+@pytest.mark.parametrize("n,v,dtype", [(40, 151552, BF16), (7, 151936, FP32), (3000, 24000, BF16), (20000, 64, BF16)])
+def test_losses_inside_an_sm_budget(n, v, dtype):
+    """On the stream of a few SMs, where the clusters take turns: the same bits."""
+    from results_b200.utils.sm_budget import SmBudget
+
+    x, y, old, adv, ref = _policy_case(n, v, dtype, 1)
+    y[n // 2] = -1
+    ids, t = torch.randint(0, v, (n, 20), device="cuda", generator=_gen(1)), torch.randn(n, 20, device="cuda", generator=_gen(2))
+    x.requires_grad_(True)
+
+    def step():
+        losses = [lz.policy_loss(x, y, old, adv, ref_logp=ref, kl_coef=0.1).loss, lz.distill_loss(x, ids, t).loss,
+                  lz.token_logprobs(x, y).sum()]
+        return losses + [torch.autograd.grad(loss * s, x)[0] for loss, s in zip(losses, (1, 2, 3))]
+
+    want = step()
+    torch.cuda.synchronize()
+    with SmBudget(0, 16) as b:
+        with torch.cuda.stream(b.stream):
+            got = step()
+        b.stream.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(want, got))
+        del got
