@@ -35,6 +35,24 @@ __host__ __device__ inline int list_bytes(int kind, int top, int hash, int views
   return kind == LZ_LOSS_DISTILL ? (top * 16 * views + hash * 4 * kListWarps + 127) / 128 * 128 : 0;
 }
 
+// Every wait for a phase of a barrier is bounded. One that gives up marks its CTA. Nobody hands on
+// what a marked CTA has of a row, so what others still receive is right; its warps leave their
+// loops and tell all CTAs of the cluster, whose other waits then give up at once unless their
+// phase is there. When all threads have left, every CTA of the cluster writes NaN over the
+// outputs and gradients of the cluster's rows. In us, without and with the looks at the mark:
+// 4096 rows of 300 KB, sums only 191 / 196, 8192 of 64 KB with DISTILL's gradient 255 / 258.
+struct WaitState {
+  unsigned long long limit;  // ns
+  int failed;                // kFailed, or from the start kNoWait: what is not there at once is given up
+};
+constexpr int kFailed = 1, kNoWait = 2;
+
+LZ_DEV void init_waits(WaitState* w, unsigned long long limit) {
+  w->limit = limit;
+  w->failed = limit == 1 ? kNoWait : 0;
+}
+LZ_DEV bool gave_up(const WaitState* w) { return *(const volatile int*)&w->failed == kFailed; }
+
 struct alignas(128) StreamShared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t parts[2], peers[2], dense[2];  // of every other row
@@ -44,7 +62,7 @@ struct alignas(128) StreamShared {
   RowHead heads[4];
   RowGrad grad[2];
   RowParams params[4];
-  int failed;
+  WaitState waits;
 };
 
 LZ_DEV void mbar_arrive(uint64_t* bar) {
@@ -69,11 +87,6 @@ LZ_DEV void mbar_expect(uint64_t* bar, uint32_t bytes) {
                : "memory");
 }
 
-// Every wait for a phase of a barrier is bounded. One that gives up says so to all CTAs of
-// the cluster, whose other waits then give up at once unless their phase is there. Whoever
-// waited in vain leaves its loop without another look at what it waited for, arrives nowhere
-// and sends nothing, so what others still receive is right. When all threads have left,
-// every CTA of the cluster writes NaN over the outputs and gradients of the cluster's rows.
 template <bool CLUSTER>
 LZ_DEV bool try_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -96,44 +109,37 @@ LZ_DEV bool try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-LZ_DEV void give_up(volatile int* failed) {
-  *failed = 1;
-  const uint32_t own = smem_addr(const_cast<int*>(failed)), ranks = cluster_size();
-  for (uint32_t rank = 0; ranks > 1 && rank < ranks; ++rank)
-    asm volatile(
-        "{\n\t.reg .b32 p;\n\t"
-        "mapa.shared::cluster.u32 p, %0, %1;\n\t"
-        "st.shared::cluster.u32 [p], 1;\n\t}" ::"r"(own),
-        "r"(rank)
-        : "memory");
-}
-
 template <bool CLUSTER>
-__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* failed, unsigned long long limit) {
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile WaitState* w) {
   unsigned long long began = 0;
-  for (uint32_t it = 1; it && limit > 1; ++it) {  // 1: what is not there at once is given up
+  for (uint32_t it = 1; it; ++it) {
     if (try_wait<CLUSTER>(bar, parity)) return true;
-    if (*failed) return false;
+    if (w->failed) break;
     if (it % 64 == 0) {
       const unsigned long long now = globaltimer();
       if (!began) began = now;
-      if (now - began > limit) break;
+      if (now - began > w->limit) break;
     }
   }
-  give_up(failed);
+  w->failed = kFailed;
   return false;
 }
 
-// By one lane.
-LZ_DEV bool lane_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned long long limit) {
-  return try_wait<false>(smem_addr(bar), parity) || wait_on<false>(smem_addr(bar), parity, failed, limit);
+// Whether the phase came; lanes of a warp may differ.
+template <bool CLUSTER>
+LZ_DEV bool ring_wait(uint64_t* bar, uint32_t parity, WaitState* w) {
+  return try_wait<CLUSTER>(smem_addr(bar), parity) || wait_on<CLUSTER>(smem_addr(bar), parity, w);
 }
 
-// By a whole warp; the same in every lane.
-template <bool CLUSTER>
-LZ_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed, unsigned long long limit) {
-  if (__all_sync(~0u, try_wait<CLUSTER>(smem_addr(bar), parity))) return true;
-  return __all_sync(~0u, wait_on<CLUSTER>(smem_addr(bar), parity, failed, limit));
+// One lane, when it or its warp has given up.
+LZ_DEV void tell_cluster(const WaitState* w) {
+  for (uint32_t rank = 0, ranks = cluster_size(); rank < ranks; ++rank)
+    asm volatile(
+        "{\n\t.reg .b32 p;\n\t"
+        "mapa.shared::cluster.u32 p, %0, %1;\n\t"
+        "st.shared::cluster.u32 [p], %2;\n\t}" ::"r"(smem_addr(&w->failed)),
+        "r"(rank), "r"(kFailed)
+        : "memory");
 }
 
 // After a wait that gave up: copies and peers' values still in flight land before the CTA ends.
@@ -177,8 +183,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
   const long long cluster = blockIdx.x / ranks, clusters = gridDim.x / ranks;
   const float c = (float)(kLog2e * (double)a.inv_temperature);
-  volatile int* const failed = &sh.failed;
-  const unsigned long long limit_ns = plan.wait_ns;
+  WaitState* const waits = &sh.waits;
   // Rows of this cluster: i = cluster, cluster + clusters, ... below `limit`, those that count first.
   const long long limit = plan.ordered ? a.rows : min(a.rows, clusters);
   const int active = plan.ordered ? *work_active(a) : 0;
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       mbar_init(&sh.used[k], 1);
     }
     fence_mbar_init();
-    *failed = 0;
+    init_waits(waits, plan.wait_ns);
   }
   if (warp == W + 1 && lane < 2) sh.heads[lane] = head_at(cluster + lane * clusters);
   cluster_sync();
@@ -226,7 +231,10 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         const RowHead next = head_at(i + clusters);
         const char* from = reinterpret_cast<const char*>(row_of<T>(a, h.row) + h.lead) + (size_t)h.first * 16;
         for (int k = 0; k < h.chunks; ++k) {
-          if (round && !lane_wait(&sh.empty[slot], (round - 1) & 1, failed, limit_ns)) goto fed;
+          if (round && !ring_wait<false>(&sh.empty[slot], (round - 1) & 1, waits)) {
+            tell_cluster(waits);
+            goto fed;
+          }
           const int vecs = min(kChunkVecs, h.count - k * kChunkVecs);
           bulk_g2s(ring + (size_t)slot * kChunk, from + (size_t)k * kChunk, vecs * 16, &sh.full[slot]);
           if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
@@ -242,11 +250,12 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     LazySum sum;
     sum.init(c);
     int done = 0;  // chunks of the row that are in `sum`
-    // Chunks [done, upto) of a row; false where one did not come.
+    // Chunks [done, upto) of a row. Where one does not come its slot is read all the same, so that a warp
+    // stays together, but not handed back to the ring.
     auto take = [&](const RowHead& h, int upto) {
       for (; done < upto; ++done) {
         const int vecs = h.count - done * kChunkVecs;
-        if (!warp_wait<false>(&sh.full[slot], round & 1, failed, limit_ns)) return false;
+        const bool came = ring_wait<false>(&sh.full[slot], round & 1, waits);
         const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk) + tid;
         if (vecs >= kChunkVecs) {
           uint4 w[kBatch];
@@ -258,27 +267,30 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         }
         if (!GRAD) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[slot]);
+          if (lane == 0 && came) mbar_arrive(&sh.empty[slot]);
         }
         if (++slot == (uint32_t)plan.slots) slot = 0, ++round;
       }
-      return true;
     };
     uint32_t turn = 0;
-    bool all_there = true;
     for (;; ++turn) {
       // The row's head is there, and its place in `warp_part` free, when the row two before it is done with.
       const int k = turn & 1;
-      if (!GRAD && turn >= 2 && !(all_there = warp_wait<false>(&sh.dense[k], ((turn - 2) >> 1) & 1, failed, limit_ns))) break;
+      if (!GRAD && turn >= 2) {
+        ring_wait<false>(&sh.dense[k], ((turn - 2) >> 1) & 1, waits);
+        __syncwarp();
+        if (gave_up(waits)) break;  // a load of the whole warp: the same in every lane
+      }
       const RowHead h = sh.heads[turn & 3];
       if (h.row < 0) break;
       const long long single = rank == 0 && tid < 2 * N ? single_of(h.lead, h.vecs, N, tid, a.vocab) : -1;
       float alone = 0.f;
       if (single >= 0) alone = Elem<T>::get(row_of<T>(a, h.row)[single]);
-      if (!(all_there = take(h, h.chunks))) break;
+      take(h, h.chunks);
       if (single >= 0) sum.take_one(alone, c);
       float m = sum.ref, all = sum.total();
       lanes_join(m, all, 32);
+      __syncwarp();
       if (lane == 0) {
         sh.warp_part[k][warp] = make_float2(m, all);
         mbar_arrive(&sh.parts[k]);
@@ -287,8 +299,10 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       done = 0;
       if (!GRAD) continue;
       const RowHead& next = sh.heads[(turn + 1) & 3];
-      if (next.row >= 0 && !(all_there = take(next, min(plan.early, next.chunks)))) break;
-      if (!(all_there = warp_wait<false>(&sh.dense[k], (turn >> 1) & 1, failed, limit_ns))) break;
+      if (next.row >= 0) take(next, min(plan.early, next.chunks));
+      ring_wait<false>(&sh.dense[k], (turn >> 1) & 1, waits);
+      __syncwarp();
+      if (gave_up(waits)) break;
       const RowGrad d = sh.grad[k];
       T* out = static_cast<T*>(a.grad) + h.row * a.vocab;
       const uint64_t c2 = pair(c, c), f2 = pair(d.f, d.f), off2 = pair(-d.ref, -d.ref);
@@ -328,7 +342,9 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
         out[single] = Elem<T>::put(d.f == 0.f ? 0.f : d.dense(alone, c));
     }
     __syncwarp();
-    if (GRAD && all_there) {
+    const bool there = !gave_up(waits);
+    if (!there && lane == 0) tell_cluster(waits);
+    if (GRAD && there) {
       if (lane == 0) mbar_arrive(&sh.parts[turn & 1]);  // the last row is written
       for (long long i = (plan.ordered ? active : 0) + cluster; i < limit; i += clusters) {
         long long r;
@@ -348,7 +364,10 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     for (uint32_t turn = mine; mine < views / 2 && row_at(cluster + (long long)turn * clusters, &r); turn += views / 2) {
       const int k = turn & (views - 1);
       if (row_at(cluster + (long long)(turn + views) * clusters, &to_come)) touch_list(a, to_come);
-      if (turn >= views && !warp_wait<false>(&sh.used[k], ((turn >> views_log2) - 1) & 1, failed, limit_ns)) break;
+      if (turn >= views && !__all_sync(~0u, ring_wait<false>(&sh.used[k], ((turn >> views_log2) - 1) & 1, waits))) {
+        if (lane == 0) tell_cluster(waits);
+        break;
+      }
       prepare_params<T, KIND>(a, row_of<T>(a, r), r, sh.params[k], view(k), hash, plan.hash, c);
       if (lane == 0) mbar_arrive(&sh.ready[k]);
       if (row_at(cluster + (long long)(turn + views / 2) * clusters, &to_come))
@@ -384,26 +403,29 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     };
     prepare(sh.heads[0], 0);
     uint32_t turn = 0;
-    bool all_there = true;
     for (;; ++turn) {
       const RowHead h = sh.heads[turn & 3];
       if (h.row < 0) break;
       const int k = turn & 1, at = turn & (views - 1), last = (turn - 1) & (views - 1);
       const RowHead later = head_at(cluster + (long long)(turn + 2) * clusters);
-      if (!(all_there = warp_wait<false>(&sh.parts[k], (turn >> 1) & 1, failed, limit_ns))) break;
+      ring_wait<false>(&sh.parts[k], (turn >> 1) & 1, waits);
       float2 v = lane < W ? sh.warp_part[k][lane] : make_float2(-INFINITY, 0.f);
       lanes_join(v.x, v.y, W);
       if (ranks > 1) {
+        __syncwarp();
+        if (gave_up(waits)) break;
         if (lane == 0) mbar_expect(&sh.peers[k], ranks * (uint32_t)sizeof(float2));
         if (lane < ranks) send_to_peer(&sh.peer_part[k][rank], v, &sh.peers[k], lane);
         __syncwarp();
-        if (!(all_there = warp_wait<true>(&sh.peers[k], (turn >> 1) & 1, failed, limit_ns))) break;
+        ring_wait<true>(&sh.peers[k], (turn >> 1) & 1, waits);
         v = lane < ranks ? sh.peer_part[k][lane] : make_float2(-INFINITY, 0.f);
         lanes_join(v.x, v.y, kMaxCluster);
       }
       RowSum n = {0.f, v.x, v.y};
+      if (KIND == LZ_LOSS_DISTILL) ring_wait<false>(&sh.ready[at], (turn >> views_log2) & 1, waits);
+      __syncwarp();
+      if (gave_up(waits)) break;
       if (!exact_ref(v.x)) n = slow_sum(row_of<T>(a, h.row), a.vocab, c);
-      if (KIND == LZ_LOSS_DISTILL && !(all_there = warp_wait<false>(&sh.ready[at], (turn >> views_log2) & 1, failed, limit_ns))) break;
       const RowParams& p = sh.params[at];
       const RowOut o = row_out<KIND>(a, p, n.norm(), c);
       const RowGrad g(o.slope, a.inv_temperature, n);
@@ -420,14 +442,17 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
       __syncwarp();
       prepare(sh.heads[(turn + 1) & 3], k ^ 1);
     }
-    if (GRAD && all_there && (all_there = warp_wait<false>(&sh.parts[turn & 1], (turn >> 1) & 1, failed, limit_ns)))
-      sparse((turn - 1) & (views - 1));
+    if (GRAD && !gave_up(waits)) ring_wait<false>(&sh.parts[turn & 1], (turn >> 1) & 1, waits);
+    __syncwarp();
+    const bool there = !gave_up(waits);
+    if (GRAD && there) sparse((turn - 1) & (views - 1));
+    if (!there && lane == 0) tell_cluster(waits);
     if (rank == 0) {
       long long r;
       for (long long i = (plan.ordered ? active : 0) + cluster + lane * clusters; i < limit; i += 32 * clusters) {
         if (!row_at(i, &r)) no_outputs<KIND>(a, r);
       }
-      if (!all_there) loss = NAN;
+      if (!there) loss = NAN;
       if (KIND != LZ_LOSS_LOGP) {  // the cluster that is done last adds the losses up, in the clusters' order
         int last = 0;
         if (lane == 0) {
@@ -448,7 +473,7 @@ __global__ void __launch_bounds__((W + kHelpers<KIND>) * 32, 1) stream_kernel(co
     __syncwarp();
   }
   cluster_sync();  // no CTA leaves while a peer may still write to it
-  if (!*failed) return;
+  if (!gave_up(waits)) return;
   drain_copies();
   for (long long i = cluster; i < limit; i += clusters) {
     long long r;
@@ -485,7 +510,7 @@ struct ChunkHead {
 struct alignas(128) GradShared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   ChunkHead heads[kMaxSlots];
-  int failed;
+  WaitState waits;
 };
 
 template <typename T, int KIND, int W>
@@ -498,7 +523,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
   char* const ring = smem + sizeof(GradShared);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const float c = (float)(kLog2e * (double)a.inv_temperature);
-  volatile int* const failed = &sh.failed;
+  WaitState* const waits = &sh.waits;
   const float up = a.upstream ? *a.upstream : 1.f;
   if (!a.fresh && up == 1.f) return;
   if (tid == 0) {
@@ -507,7 +532,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
       mbar_init(&sh.empty[s], W);
     }
     fence_mbar_init();
-    *failed = 0;
+    init_waits(waits, limit_ns);
   }
   __syncthreads();
   const int per_row = (int)((a.vocab / N + kChunkVecs - 1) / kChunkVecs);  // chunks of a row, the last of them maybe empty
@@ -547,7 +572,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
       bool free = true;
       for (int l = 0; l < 32 && first + (long long)l * gridDim.x < all; ++l) {
         if (lane == l) {
-          free = !round || lane_wait(&sh.empty[slot], (round - 1) & 1, failed, limit_ns);
+          free = !round || ring_wait<false>(&sh.empty[slot], (round - 1) & 1, waits);
           if (free) {
             sh.heads[slot] = h;
             if (h.f != 0.f && h.vecs > 0) bulk_g2s(ring + (size_t)slot * kChunk, from, h.vecs * 16, &sh.full[slot]);
@@ -563,7 +588,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
   } else {
     uint32_t slot = 0, round = 0;
     for (long long g = blockIdx.x; g < all; g += gridDim.x) {
-      if (!warp_wait<false>(&sh.full[slot], round & 1, failed, limit_ns)) break;
+      if (!__all_sync(~0u, ring_wait<false>(&sh.full[slot], round & 1, waits))) break;
       const ChunkHead& h = sh.heads[slot];
       const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)slot * kChunk) + tid;
       uint4* o = static_cast<uint4*>(h.out) + tid;
@@ -610,7 +635,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
     }
   }
   __syncthreads();
-  if (!*failed) return;
+  if (!gave_up(waits)) return;
   drain_copies();
   for (long long g = blockIdx.x; g < all; g += gridDim.x) {  // this CTA's chunks are NaN, not stale
     const long long r = g / per_row, piece = g % per_row;

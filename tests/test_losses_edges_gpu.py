@@ -391,3 +391,14 @@ def test_losses_inside_an_sm_budget(n, v, dtype):
         b.stream.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(want, got))
         del got
+
+
+@pytest.mark.parametrize("v", [40, 40000])
+def test_a_small_kl_beside_a_far_ratio(v):
+    """A ratio beyond fp32 at advantage zero, and a reference that is close: the gradient is the KL's."""
+    x, y, _, _, _ = _policy_case(3, v, FP32, 1)
+    lp = oracle.logp64(x, y[:, None], 1.0)[0][:, 0]
+    ref = (lp + torch.tensor([1e-4, 1e-2, -1.0], device="cuda")).float()
+    old, adv = (lp - 120).float(), torch.zeros(3, device="cuda")
+    _check_policy(x, y, old, adv, ref, beta=0.5)
+    _check_policy(x, y, old, adv, ref, beta=0.5, upstream=-3.0)
