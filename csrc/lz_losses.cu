@@ -596,8 +596,8 @@ int run(LzLossArgs* a, cudaStream_t s, bool forward) {
   }
   const OnDevice on(a->device);
   LZ_CUDA_TRY(on.rc);
-  if (forward) a->capture = capture_of(s);
-  else if (!a->fresh && a->capture != capture_of(s)) return LZ_LOSS_APART;
+  if (forward && a->grad) a->capture = capture_of(s);
+  if (!forward && !a->fresh && a->capture != capture_of(s)) return LZ_LOSS_APART;
   switch (a->dtype) {
     case LZ_F32: return run_kind<float>(a, s, forward);
     case LZ_F16: return run_kind<__half>(a, s, forward);

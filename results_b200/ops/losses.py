@@ -162,12 +162,11 @@ def _check_denom(what: str, denom, device):
 
 def _check_modes(what: str, *tensors: torch.Tensor | None) -> None:
     """CUDA tensors: what goes past autograd functions would be lost in the kernels."""
-    if torch._C._get_tracing_state() is not None:
+    if _is_tracing():
         raise RuntimeError(f"{what}: a call with CUDA tensors cannot be traced")
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{what}: no forward-mode derivative for CUDA tensors")
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: no forward-mode derivative for CUDA tensors")
 
 
 # ---- native calls ---------------------------------------------------------------------------------------
@@ -199,18 +198,19 @@ def _rows_of(x: torch.Tensor):
 
 _lib = None
 _saved_hooks = torch._C._autograd._top_saved_tensors_default_hooks
+_is_tracing = torch._C._is_tracing
 
 _APART = 1  # LZ_LOSS_APART
 
 
-def _launch(fn: str, a, what: str) -> bool:
+def _launch(fn: str, a) -> bool:
     """False: nothing ran, the forward pass belongs to another graph capture."""
     global _lib
     if _lib is None:
         _lib = _native.cuda()
     rc = getattr(_lib, fn)(C.byref(a), torch._C._cuda_getCurrentRawStream(a.device))
     if rc and rc != _APART:
-        _native.check(rc, what)
+        _native.check(rc, "preference loss" if fn == "lz_loss_pairs" else _NAMES[a.kind])
     return not rc
 
 
@@ -227,9 +227,10 @@ class _Call:
         self.grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if fused else None
         self.out, self.shape = out, logits.shape
         self.keep = (x, ids, work) if teacher is None else (x, ids, work, teacher)
-        a = self.args = _LossArgs(
-            x.data_ptr(), outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(self.grad), ids.data_ptr())
-        a.work, a.inv_temperature, a.kind = work.data_ptr(), 1.0 / temperature, kind
+        at = self.at = x.data_ptr(), ids.data_ptr(), work.data_ptr()
+        self.strides = x.stride() if outer_stride or inner_stride != x.shape[-1] else None  # None: contiguous
+        a = self.args = _LossArgs(at[0], outer_stride, inner_stride, inner, n, x.shape[-1], _ptr(self.grad), at[1])
+        a.work, a.inv_temperature, a.kind = at[2], 1.0 / temperature, kind
         a.dtype, a.ids64, a.device = _DTYPES[x.dtype], ids.dtype is torch.int64, dev.index
         a.logp = _ptr(logp)
         if kind == LOGP:
@@ -247,7 +248,7 @@ class _Call:
             a.teacher, a.teacher_dtype, a.top = teacher.data_ptr(), _DTYPES[teacher.dtype], ids.shape[-1]
 
     def forward(self) -> None:
-        _launch("lz_loss_forward", self.args, _NAMES[self.args.kind])
+        _launch("lz_loss_forward", self.args)
 
     def set_upstream(self, a, g: int, saved) -> None:
         """`g`: address of the upstream gradient, of each row's log-probability or of the loss."""
@@ -264,16 +265,17 @@ class _Call:
         grad = self.__dict__.pop("grad", None)
         if g.dtype is not torch.float32 or not g.is_contiguous():
             g = g.to(torch.float32).contiguous()
-        if self.hooked or x.data_ptr() != a.logits or x.stride() != self.strides or saved[1].data_ptr() != a.ids or \
-                saved[2].data_ptr() != a.work or (a.kind == DISTILL and saved[3].data_ptr() != a.teacher):
+        if self.hooked or (x.data_ptr(), saved[1].data_ptr(), saved[2].data_ptr()) != self.at or \
+                not (x.is_contiguous() if self.strides is None else x.stride() == self.strides) or \
+                (a.kind == DISTILL and saved[3].data_ptr() != a.teacher):
             saved = self.came_back(a, saved)
             x = saved[0]
         self.set_upstream(a, g.data_ptr(), saved)
-        if grad is None or not _launch("lz_loss_backward", a, _NAMES[a.kind]):
+        if grad is None or not _launch("lz_loss_backward", a):
             a.fresh = 1
             grad = torch.empty(self.shape, dtype=x.dtype, device=x.device)
             a.grad = grad.data_ptr()
-            _launch("lz_loss_backward", a, _NAMES[a.kind])
+            _launch("lz_loss_backward", a)
         return grad
 
     def came_back(self, a, saved):
@@ -301,7 +303,7 @@ class _Loss(torch.autograd.Function):
     def forward(ctx, logits, call):
         call.forward()
         ctx.save_for_backward(*call.keep)
-        call.strides, call.hooked = call.keep[0].stride(), _saved_hooks(True) is not None
+        call.hooked = _saved_hooks(True) is not None
         ctx.call, out = call, call.out
         call.keep = call.out = None  # the output leads here: it may not be held from here
         return out
@@ -344,7 +346,7 @@ class _PairsCall(_Call):
 
     def forward(self) -> None:
         super().forward()
-        _launch("lz_loss_pairs", self.pairs, "preference loss")
+        _launch("lz_loss_pairs", self.pairs)
         self.alive = None
 
     def came_back(self, a, saved):
@@ -464,7 +466,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     temperature = _check_temperature(what, temperature)
     if not logits.is_cuda:
         return _cpu_token_logprobs(logits, tokens, temperature)
-    _check_modes(what, logits)
+    if _is_tracing() or forward_ad._current_level >= 0:
+        _check_modes(what, logits)
     logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
     return _run(_Call(LOGP, logits, tokens, temperature, logp, logp), logits, _needs_grad(logits))
 
@@ -501,7 +504,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
          "temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
     if not logits.is_cuda:
         return PolicyLoss(*_cpu_policy_loss(logits, tokens, rows, p))
-    _check_modes(what, logits, old_logp, advantages, ref_logp, weights, denom)
+    if _is_tracing() or forward_ad._current_level >= 0:
+        _check_modes(what, logits, old_logp, advantages, ref_logp, weights, denom)
     needs_grad, old = _needs_grad(logits), rows[0]  # old_logp: contiguous, fp32, of the tokens' shape
     logp, clipped = torch.empty_like(old), torch.empty_like(old, dtype=torch.bool)
     kl = None if ref_logp is None else torch.empty_like(old)
@@ -548,7 +552,8 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, *, ref_logp: tor
     if not logits.is_cuda:
         loss, rewards = _cpu_preference_loss(logits, tokens, ref, cu_seqlens, p)
     else:
-        _check_modes(what, logits, ref_logp)
+        if _is_tracing() or forward_ad._current_level >= 0:
+            _check_modes(what, logits, ref_logp)
         call = _PairsCall(logits, tokens, ref, cu_seqlens, p)
         loss, rewards = _run(call, logits, _needs_grad(logits)), call.rewards
     return PreferenceLoss(loss, *rewards.split(p["pairs"]))
@@ -586,7 +591,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     p = {"temperature": _check_temperature(what, temperature), "denom": _check_denom(what, denom, dev)}
     if not logits.is_cuda:
         return DistillLoss(*_cpu_distill_loss(logits, ids, teacher, weights, p))
-    _check_modes(what, logits, teacher_logits, weights, denom)
+    if _is_tracing() or forward_ad._current_level >= 0:
+        _check_modes(what, logits, teacher_logits, weights, denom)
     needs_grad = _needs_grad(logits)
     kl = torch.empty(shape, dtype=torch.float32, device=dev)
     call = _Call(DISTILL, logits, ids, p["temperature"], kl.new_empty(()), None, kl, None, (None, None, None, weights), teacher,

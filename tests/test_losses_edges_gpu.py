@@ -344,10 +344,10 @@ def test_waits_that_give_up(monkeypatch, wait_ns, n, v, dtype):
     want = step()
     launch = losses._launch
 
-    def short(fn, args, what):
+    def short(fn, args):
         if fn != "lz_loss_pairs":
             args.wait_ns = wait_ns
-        return launch(fn, args, what)
+        return launch(fn, args)
 
     monkeypatch.setattr(losses, "_launch", short)
     got = step()
