@@ -11,10 +11,14 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 // CTAs an SM: 64 registers a thread. With four blocks of 256 the sums of 8192 rows of
-// 64 KB took 110 us, not 96.
+// 64 KB took 110 us, not 96. Some kernels spill for it (policy's gradient by parts of a warp
+// 208 bytes). Six CTAs need no spill: policy steps of 262144 x 256 took 100 us, not 109, of 8192 x
+// 16384 128, not 133, but sums alone 62, not 59, and 72, not 68, and DISTILL's of 8192 x 4000 52, not 50.
 constexpr int kRowCtas = 8;
 constexpr long long kWarpBytes = 8192;  // of the rows that a warp has at a time
-constexpr long long kHeadRows = 2048;   // more are the head's cluster's
+// More are the head's cluster's. A policy step of 24000 columns, one CTA against the cluster: 1024 rows
+// 34.7 / 36.7 us, 2048 61.6 / 61.3, 3000 81.6 / 80.2, 8192 191.6 / 187.0.
+constexpr long long kHeadRows = 2048;
 
 template <typename V>
 LZ_DEV V block_sum(V v, V* red, int warps) {

@@ -40,7 +40,8 @@ __host__ __device__ inline int list_bytes(int kind, int top, int hash, int views
 // loops and tell all CTAs of the cluster, whose other waits then give up at once unless their
 // phase is there. When all threads have left, every CTA of the cluster writes NaN over the
 // outputs and gradients of the cluster's rows. In us, without and with the looks at the mark:
-// 4096 rows of 300 KB, sums only 191 / 196, 8192 of 64 KB with DISTILL's gradient 255 / 258.
+// 1024 rows of 608 KB with policy's gradient 221 / 223, 600 of 200 KB with DISTILL's 65.6 / 67.7,
+// sums only 1 row of 300 KB 6.6 / 6.9, 4096 rows 191 / 195.
 struct WaitState {
   unsigned long long limit;  // ns
   int failed;                // kFailed, or from the start kNoWait: what is not there at once is given up
@@ -653,13 +654,19 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) stream_grad_kernel(const __gr
 
 // Whether rows are streamed: not small, and each row and its gradient at the same
 // offset from a 16-byte border. A row costs a cluster some 5000 cycles besides its
-// bytes, which the many teams of row_kernel hide better
-// while rows are short; it reads a row that outgrows the caches a second time. In
-// us, bf16, streamed against teams: 8192 rows of 64 KB, sums only 130 / 96, 4096 of
-// 300 KB 194 / 204; 8192 with the policy's gradient 32 KB 171 / 140, 64 KB 208 / 259;
-// with DISTILL's of 64 entries 48 KB 201 / 218, 64 KB 236 / 287, but 1024 rows of
-// 64 KB 48 / 42, of 100 KB 63 / 70; the gradient alone, 1024 rows of 64 KB 25 / 21, 8192 rows of 100 KB 256 / 266. Few rows are
-// streamed whatever their length, since a cluster splits them.
+// bytes, which the many teams of row_kernel hide better while rows are short; it
+// reads a row that outgrows the caches a second time. Few rows are streamed from
+// 16 KB on, since a cluster splits them. In us, bf16, streamed against teams:
+//   policy's gradient: 64 rows of 16 KB 15 / 14, of 32 KB 14 / 16, of 64 KB 16 / 21; 1024 of 48 KB 35 / 33, of
+//     64 KB 42 / 43, of 80 KB 49 / 56; 8192 of 40 KB 180 / 162, of 48 KB 187 / 194, of 64 KB 208 / 266
+//   DISTILL's, 64 entries: 64 rows of 32 KB 21 / 18, of 80 KB 21 / 23; 1024 of 72 KB 56 / 52, of 80 KB 57 / 60; 4096
+//     of 40 KB 139 / 100, of 56 KB 139 / 138, of 64 KB 146 / 159. Long lists bound the streamed rows: 4096
+//     of 64 KB with 128 entries 244 / 163
+//   sums only: 64 rows of 64 KB 10 / 10, of 160 KB 10 / 14; LOGP 1024 of 128 KB 36 / 33, of 300 KB 62 / 62, of 600 KB
+//     105 / 111, 4096 of 300 KB 220 / 211; policy 2048 of 128 KB 62 / 61, of 200 KB 80 / 82, of 400 KB 140 / 156
+//   the gradient alone: 1024 rows of 64 KB 25 / 21, 8192 of 100 KB 256 / 266
+// The borders are round numbers; next to them the other side is up to 10 % faster, for DISTILL of 4096
+// rows and more from 40 to 52 KB up to 28 %.
 template <typename T>
 bool streams(const LzLossArgs* a, bool forward, bool grad) {
   const long long size = sizeof(T), row = a->vocab * size;
@@ -703,6 +710,9 @@ int plan_as(const LzLossArgs* a, LzStreamPlan* l) {
     }
     known[a->device].store(true, std::memory_order_release);
   }
+  // CTAs a row: the fewest bytes by the busiest cluster, a row's exchange counted as 50 KB. In us with 0 / 25 / 50 /
+  // 200 KB, policy's gradient: 515 rows of 64 KB 38.4 / 32.8 / 32.8 / 32.7, 4000 of 200 KB 284 / 272 / 274 / 273, 300
+  // of 120 KB 32.8 / 32.8 / 30.8 / 31.2.
   double best = 0.0;
   int chunks = 0;
   long long part = 0;

@@ -9,10 +9,12 @@ student computes between its output head and its backward pass.
 
 ``logits`` is ``[..., vocab]`` in bf16, fp16 or fp32, ``tokens`` its leading
 shape in int32 or int64. Leading dimensions may have any strides (``logits[:, :-1]``
-is read in place); a vocabulary that is not contiguous is copied. A negative
-token marks a row that does not count (prompt, padding): its logits are not
-read, its outputs and its gradient are zero. The same holds for rows of weight
-zero. A token or teacher id beyond the vocabulary makes the row (and the loss) NaN.
+is read in place; gradients are fastest where rows start at the same offset from
+a 16-byte border as in a contiguous tensor); a vocabulary that is not contiguous
+is copied. A negative token marks a row that does not count (prompt, padding):
+its logits are not read, its outputs and its gradient are zero. The same holds
+for rows of weight zero. A token or teacher id beyond the vocabulary, or NaN or
++inf among a teacher's entries, makes a row that counts (and the loss) NaN.
 
 Sums and log-probabilities are held in 32 bits or more and a gradient is
 rounded once, to the logits' type. Results do not depend on timing: the same
