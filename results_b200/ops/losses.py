@@ -29,7 +29,8 @@ to keep the cheaper way, and capture both passes into one CUDA graph: a backward
 pass captured apart computes the gradient anew at every replay. The logits must
 not be changed before the backward pass. CUDA tensors run the kernels in
 csrc/lz_losses.cu on the current stream of their device, with a first derivative
-in the logits by the backward pass (no second one, no forward mode, no tracing);
+in the logits by the backward pass (no second one, no forward mode, no tracing;
+inside a function that torch.compile takes they run as they are);
 CPU tensors run the definitions in 64-bit torch operations.
 """
 from __future__ import annotations
@@ -202,12 +203,19 @@ _lib = None
 _saved_hooks = torch._C._autograd._top_saved_tensors_default_hooks
 _is_tracing = torch._C._is_tracing
 
+def _as_it_is() -> None:
+    """A function that begins with this is run by torch.compile as it is: it raises while the compiler traces it."""
+    if torch.compiler.is_dynamo_compiling():
+        raise RuntimeError("native calls are not compiled")
+
+
 _APART = 1  # LZ_LOSS_APART
 
 
 def _launch(fn: str, a) -> bool:
     """False: nothing ran, the forward pass belongs to another graph capture."""
     global _lib
+    _as_it_is()
     if _lib is None:
         _lib = _native.cuda()
     rc = getattr(_lib, fn)(C.byref(a), torch._C._cuda_getCurrentRawStream(a.device))
@@ -222,6 +230,7 @@ class _Call:
 
     def __init__(self, kind, logits, ids, temperature, out, logp=None, kl=None, clipped=None,
                  rows=None, teacher=None, denom=None, numbers=(0.0, 0.0, 0.0), fused=False):
+        _as_it_is()
         x, outer_stride, inner_stride, inner, n = _rows_of(logits)
         dev = x.device
         work = torch.empty(_HEAD + _PER_ROW * n, dtype=torch.float64, device=dev)
@@ -263,6 +272,7 @@ class _Call:
         """The gradient is handed out once: a second pass over a retained graph
         writes into memory of its own, and so does a pass that was captured
         apart from the forward pass."""
+        _as_it_is()
         a, x = _LossArgs.from_buffer_copy(self.args), saved[0]  # other threads may be here too
         grad = self.__dict__.pop("grad", None)
         if g.dtype is not torch.float32 or not g.is_contiguous():
@@ -332,6 +342,7 @@ class _PairsCall(_Call):
     """The log-probabilities and, from them, the preference loss."""
 
     def __init__(self, logits, tokens, ref, offsets, p):
+        _as_it_is()
         dev, rows, pairs = logits.device, tokens.numel(), p["pairs"]
         logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
         super().__init__(LOGP, logits, tokens, p["temperature"], logp, logp)

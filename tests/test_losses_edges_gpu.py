@@ -402,3 +402,19 @@ def test_a_small_kl_beside_a_far_ratio(v):
     old, adv = (lp - 120).float(), torch.zeros(3, device="cuda")
     _check_policy(x, y, old, adv, ref, beta=0.5)
     _check_policy(x, y, old, adv, ref, beta=0.5, upstream=-3.0)
+
+
+def test_calls_inside_a_compiled_function():
+    """The compiler runs them as they are (its eager backend: nothing else of the function matters here)."""
+    w, h = torch.randn(64, 1000, device="cuda", generator=_gen(1)), torch.randn(8, 64, device="cuda", generator=_gen(2))
+    w.requires_grad_(True)
+    y, z = torch.arange(8, device="cuda"), torch.zeros(8, device="cuda")
+    ids, t = y[:, None] + torch.arange(5, device="cuda"), torch.randn(8, 5, device="cuda", generator=_gen(3))
+    for f in (lambda w: lz.policy_loss(h @ w, y, z - 7, z + 1, ref_logp=z - 7, kl_coef=0.1).loss * 2,
+              lambda w: -lz.token_logprobs(h @ w, y).mean(), lambda w: lz.distill_loss(h @ w, ids, t).loss,
+              lambda w: lz.preference_loss((h @ w).view(2, 4, 1000), y.view(2, 4)).loss):
+        c = torch.compile(f, backend="eager")
+        assert torch.equal(c(w), f(w))
+        assert torch.equal(torch.autograd.grad(c(w), w)[0], torch.autograd.grad(f(w), w)[0])
+        with torch.no_grad():
+            assert torch.equal(c(w), f(w))
